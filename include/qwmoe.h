@@ -50,17 +50,22 @@ extern "C" {
 /* ggml_type values used on the path (ggml/include/ggml.h:390-416). */
 enum qwmoe_type {
     QWMOE_TYPE_F32 = 0,
+    QWMOE_TYPE_F16 = 1,
     QWMOE_TYPE_Q8_0 = 8,
     QWMOE_TYPE_Q4_K = 12,
     QWMOE_TYPE_Q6_K = 14,
     QWMOE_TYPE_Q8_K = 15,
-    QWMOE_TYPE_I32 = 26
+    QWMOE_TYPE_I32 = 26,
+    QWMOE_TYPE_BF16 = 30
 };
 
 /* Device status bits (qwmoe_device_status). */
 #define QWMOE_STATUS_TOPK_TIE_SORT 1   /* a top-k tie was resolved by the exact std::sort replay (informational) */
 #define QWMOE_STATUS_BAD_ID 2          /* an ids entry was outside [0, n_as) and was skipped */
-#define QWMOE_STATUS_BAD_SLOT 4        /* a slot table entry was outside [0, n_slots) and was skipped */
+#define QWMOE_STATUS_BAD_SLOT 4        /* a slot table entry was outside [0, n_slots) and was skipped; a cache slot or
+                                          page was outside its pool */
+#define QWMOE_STATUS_NO_PAGES 16       /* qwmoe_kv_plan: a request got no pages (too few are free) */
+#define QWMOE_STATUS_BAD_SEQ 32        /* a request's lengths do not fit the call (qwmoe_kv_plan, qwmoe_attn_kv_q4) */
 
 /* ---- library ------------------------------------------------------------ */
 
@@ -509,6 +514,95 @@ int qwmoe_layer_stack_kernel_t1(qwmoe_layer_stack * s);
  * qwmoe_decode_stack_status: 1 top-k tie replayed, 8 a wait timed out plus the
  * exchange, 16 a slot out of range), 0 for the per-layer chain. */
 int qwmoe_layer_stack_status(void * stream, qwmoe_layer_stack * s, int32_t * status_out, int clear);
+
+/* ---- a batch's key/value cache, in pages and in 4 bits ------------------------- */
+
+/* The caches of one layer for many requests of different lengths, in caller memory:
+ * n_pages pages of page_tokens tokens (a power of two, 32 .. 4096), each
+ * [n_head_kv][page_tokens / 32 cells]; keys and values lie in one cell of 36 D bytes
+ * per 32 tokens of a kv head (D = n_embd_head = 64, 128 or 256):
+ *   key codes 16 D | key scales 2 D | value codes 16 D | value scales 2 D.
+ * A block is 32 consecutive dimensions of one token's head.  With m its value of
+ * largest magnitude (the positive one of two): scale d = f16(m / -8), at most
+ * 65504 in magnitude; code = x / d to the nearest integer (ties to even), clamped to
+ * -8 .. 7, plus 8; the block then stands for d (code - 8).  A block with a NaN or
+ * an infinity gets a NaN scale: all its 32 values read as NaN.
+ * Place of token 4 g + i (0 <= g, i < 4) of the cell's 16-token half u, block b of
+ * NB = D / 32:
+ *   key codes    dword ((16 u + 4 g + i) 4 + q) NB + b: dims 32 b + 8 q + j, j = 0 .. 7,
+ *                at nibble j / 2 + 4 (j % 2), nibble 0 the lowest;
+ *   value codes  byte i of dword ((((b / 2) 16 + j) 4 + g) 2 + b % 2) 2 + u: dim 32 b + j in
+ *                the low nibble, dim 32 b + 16 + j in the high one;
+ *   scales       half ((4 u + g) NB + b) 4 + i.
+ * A slot is page * page_tokens + place in the page.  No counterpart in the
+ * reference, whose caches are dense f16 rows of one request
+ * (core/runtime.cpp:494-520); 4.5 bits a value are 0.28 of those bytes. */
+typedef struct qwmoe_kv_q4 {
+    int64_t n_head_kv, n_embd_head, page_tokens, n_pages;
+    void * data;               /* n_pages * qwmoe_kv_q4_page_bytes, 16-byte aligned; need not be cleared */
+} qwmoe_kv_q4;
+
+/* Bytes of a page; 0 for a shape the cache does not take. */
+size_t qwmoe_kv_q4_page_bytes(int64_t n_head_kv, int64_t n_embd_head, int64_t page_tokens);
+
+/* One round of a batch's bookkeeping, from its lengths alone, on the device.
+ * Request i of n_seq (at most 4096) holds the pages of held[i] tokens, the first
+ * ceil(held / page_tokens) entries of its row of page_table [n_seq][table_width].
+ * It keeps the first past[i] <= held[i] tokens (fewer after rejected drafts, 0 when it
+ * ends) and adds n_new[i] >= 0.  Pages it lacks then come off the ring of free
+ * pages, in the order of the requests; pages it no longer needs go back to it.
+ *   ring      i32 [n_pages]: free pages at ring[k % n_pages], head <= k < tail; pages
+ *             put back are written from tail on
+ *   counters  i64 {head, tail}; counters_out (another buffer) receives the next ones
+ *   seq_start i32 [n_seq + 1]: prefix sums of n_new; seq_len i32 [n_seq]: past + n_new
+ *   slot      i64 [n_tokens], pos i32 [n_tokens]: of every new token row, request by
+ *             request; rows behind the last one get -1 (a captured call keeps n_tokens)
+ * page_table and ring are updated in place; entries that neither rule names stay.  A
+ * request that the free pages do not serve, and every later one that needs pages,
+ * keeps its pages as they are: seq_len 0, slots -1 (QWMOE_STATUS_NO_PAGES).  So does one
+ * whose lengths are negative, past > held, wider than the table, or whose rows end
+ * behind n_tokens (QWMOE_STATUS_BAD_SEQ).  A page outside [0, n_pages) gives
+ * slot -1 (QWMOE_STATUS_BAD_SLOT).  No workspace. */
+int qwmoe_kv_plan(void * stream, const int32_t * held, const int32_t * past, const int32_t * n_new, int64_t n_seq,
+                  int64_t page_tokens, int64_t n_pages, int32_t * page_table, int64_t table_width, int32_t * ring,
+                  const int64_t * counters, int64_t * counters_out, int64_t n_tokens, int32_t * seq_start,
+                  int32_t * seq_len, int64_t * slot, int32_t * pos);
+
+/* Key and value rows (n_tokens rows of n_head_kv * D values of `type` F32, F16 or BF16,
+ * k_nb1 / v_nb1 bytes apart) quantized into the cache at slot[t].  A negative slot
+ * passes its row over; one outside the pool is skipped (QWMOE_STATUS_BAD_SLOT).  The
+ * slots of a call are distinct: of two rows with one slot, each block is either
+ * row's or, code by code, a mixture.  Rows and strides 16-byte aligned.  No workspace. */
+int qwmoe_kv_q4_store(void * stream, const qwmoe_kv_q4 * cache, int type, const void * k, size_t k_nb1,
+                      const void * v, size_t v_nb1, const int64_t * slot, int64_t n_tokens);
+
+/* The reverse: d (code - 8) of the rows at slot[t], rounded to `type`.  A row whose slot
+ * is negative or outside the pool (QWMOE_STATUS_BAD_SLOT) is left as it was.  A slot may
+ * occur more than once. */
+int qwmoe_kv_q4_load(void * stream, const qwmoe_kv_q4 * cache, int type, void * k, size_t k_nb1, void * v,
+                     size_t v_nb1, const int64_t * slot, int64_t n_tokens);
+
+/* Causal attention of a batch over the cache: request i's token rows are
+ * seq_start[i] .. seq_start[i + 1] - 1 of q, its last n = that many tokens of seq_len[i]
+ * (all in the cache by then); row t's head h attends to keys 0 .. seq_len - n + t of kv head
+ * h / (n_head / n_head_kv):  out = sum_j softmax_j(kq_scale q . k_j) v_j.
+ *   q, out: `type` (F32, F16, BF16) [n_tokens][n_head][D], tokens q_nb1 / out_nb1 bytes
+ *   apart, 16-byte aligned, not the same buffer; kq_scale > 0, or 0 for 1 / sqrt(D)
+ *   max_new, max_len: upper bounds of n and of seq_len (they size the launch: a
+ *   captured call keeps them); max_len <= table_width * page_tokens < 2^31
+ * A row that sees no key (seq_len 0, or n > seq_len) gets zeros; rows from
+ * seq_start[n_seq] on are left as they were.  A request beyond a bound gets zeros
+ * (QWMOE_STATUS_BAD_SEQ); keys of a page outside the pool count as masked
+ * (QWMOE_STATUS_BAD_SLOT).  Sums, the softmax's statistics and the products with f32 rows are
+ * in 32 bits (f32 rows enter the matrix cores as two f16 parts each); for F16 and BF16
+ * rows the unnormalized weights are rounded to f16 before the sum over the values.  The
+ * order of the sums follows max_new, max_len, n_seq and n_tokens, never the run.
+ * Workspace where the keys are split over workgroups (few rows, long max_len): per split
+ * n_tokens * n_head * (D + 2) floats, as many splits as fit. */
+int qwmoe_attn_kv_q4(void * stream, const qwmoe_kv_q4 * cache, int type, const void * q, size_t q_nb1,
+                     int64_t n_head, const int32_t * page_table, int64_t table_width, const int32_t * seq_start,
+                     const int32_t * seq_len, int64_t n_seq, int64_t n_tokens, int64_t max_new, int64_t max_len,
+                     float kq_scale, void * out, size_t out_nb1);
 
 /* ---- expert slot table (host) ------------------------------------------------ */
 

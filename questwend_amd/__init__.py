@@ -16,9 +16,11 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libqwmoe.so"
 
 F32, Q8_0, Q4_K, Q6_K, Q8_K, I32 = 0, 8, 12, 14, 15, 26
+F16, BF16 = 1, 30
 BLOCK = {Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210), Q8_K: (256, 292), F32: (1, 4)}
 
 STATUS_TOPK_TIE_SORT, STATUS_BAD_ID, STATUS_BAD_SLOT = 1, 2, 4
+STATUS_NO_PAGES, STATUS_BAD_SEQ = 16, 32
 
 
 class QwmoeError(RuntimeError):
@@ -83,6 +85,13 @@ class GdnLayer(C.Structure):
     ]
 
 
+class KvQ4(C.Structure):
+    """Mirror of ``qwmoe_kv_q4`` (include/qwmoe.h)."""
+
+    _fields_ = [("n_head_kv", C.c_int64), ("n_embd_head", C.c_int64), ("page_tokens", C.c_int64), ("n_pages", C.c_int64),
+                ("data", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every exported symbol of include/qwmoe.h
 P, I64, SZ, I, F, U64 = C.c_void_p, C.c_int64, C.c_size_t, C.c_int, C.c_float, C.c_uint64
 SIGNATURES = {
@@ -115,6 +124,11 @@ SIGNATURES = {
     "qwmoe_attn_seg": (I, [P, P, P, I64, I64, F, P, P]),
     "qwmoe_gdn_seg": (I, [P, P, P, I64, F, P, P]),
     "qwmoe_decoder_layer": (I, [P, P, P, P, I64, I64, F, P, P, P]),
+    "qwmoe_kv_q4_page_bytes": (SZ, [I64, I64, I64]),
+    "qwmoe_kv_plan": (I, [P, P, P, P, I64, I64, I64, P, I64, P, P, P, I64, P, P, P, P]),
+    "qwmoe_kv_q4_store": (I, [P, P, I, P, SZ, P, SZ, P, I64]),
+    "qwmoe_kv_q4_load": (I, [P, P, I, P, SZ, P, SZ, P, I64]),
+    "qwmoe_attn_kv_q4": (I, [P, P, I, P, SZ, I64, P, I64, P, P, I64, I64, I64, I64, F, P, SZ]),
     "qwmoe_decode_stack_create": (I, [P, I, F, P]),
     "qwmoe_decode_stack_run": (I, [P, P, P, P, P, P, P]),
     "qwmoe_decode_stack_status": (I, [P, P, P, I]),

@@ -17,6 +17,7 @@
 #include "qw_kernels.hpp"
 #include "qw_sort.hpp"
 #include "qw_decode.hpp"
+#include "qw_kv_q4.hpp"
 
 namespace {
 
@@ -972,6 +973,163 @@ int qwmoe_decoder_layer(void* stream, const qwmoe_attn_layer* attn, const qwmoe_
     // h_new = moe_out + attn_resid (build_segB, core/runtime.cpp:2087)
     if (rc == QWMOE_OK) rc = qw::launch_add_rms_norm_mul(moe_out, resid, h_out, nullptr, H, T, 0.0f, nullptr, S(stream));
     return rc;
+}
+
+// ---- the paged 4-bit cache -------------------------------------------------------
+
+namespace {
+
+int kv_shift(int64_t page_tokens) {   // log2, -1 where the cache does not take it
+    for (int s = 5; (int64_t(1) << s) <= qw::KV_MAX_PAGE; ++s)
+        if (page_tokens == int64_t(1) << s) return s;
+    return -1;
+}
+bool kv_shape_ok(int64_t nk, int64_t D, int64_t page_tokens) {
+    return nk > 0 && nk <= 4096 && (D == 64 || D == 128 || D == 256) && kv_shift(page_tokens) >= 0;
+}
+size_t kv_type_size(int type) {
+    return type == QWMOE_TYPE_F32 ? 4 : type == QWMOE_TYPE_F16 || type == QWMOE_TYPE_BF16 ? 2 : 0;
+}
+int kv_cache(const qwmoe_kv_q4* c, qw::KvQ4& k) {
+    if (!c || !c->data || c->n_head_kv <= 0 || c->n_embd_head <= 0 || c->page_tokens <= 0 || c->n_pages <= 0)
+        return QWMOE_ERR_INVALID_ARG;
+    if (!kv_shape_ok(c->n_head_kv, c->n_embd_head, c->page_tokens) || c->n_pages > 0x7fffffff ||
+        ((uintptr_t) c->data & 15))
+        return QWMOE_ERR_UNSUPPORTED;
+    k.data = (uint8_t*) c->data;
+    k.n_head_kv = (int) c->n_head_kv;
+    k.D = (int) c->n_embd_head;
+    k.page_shift = kv_shift(c->page_tokens);
+    k.n_pages = c->n_pages;
+    return QWMOE_OK;
+}
+// Rows of n values of `size` bytes, nb1 bytes apart, read and written 16 bytes at a time.
+int kv_rows(const void* p, size_t nb1, int64_t n, size_t size) {
+    if (!p || nb1 < (size_t) n * size) return QWMOE_ERR_INVALID_ARG;
+    return ((uintptr_t) p & 15) || nb1 % 16 ? QWMOE_ERR_UNSUPPORTED : QWMOE_OK;
+}
+// The status word and the workspace are the library device's: it has to be the current one.
+int kv_ready() {
+    if (!g_lib.ready) return QWMOE_ERR_NOT_INITIALIZED;
+    int cur = -1;
+    if (hipGetDevice(&cur) != hipSuccess) return QWMOE_ERR_HIP;
+    return cur == g_lib.device ? QWMOE_OK : QWMOE_ERR_INVALID_ARG;
+}
+int kv_rows_args(const qwmoe_kv_q4* cache, int type, const void* k, size_t k_nb1, const void* v, size_t v_nb1,
+                 const int64_t* slot, int64_t T, qw::KvRowsArgs& a) {
+    int rc;
+    if ((rc = kv_cache(cache, a.c))) return rc;
+    const size_t size = kv_type_size(type);
+    if (!size) return QWMOE_ERR_UNSUPPORTED;
+    const int64_t n = cache->n_head_kv * cache->n_embd_head;
+    if (!slot || T < 0) return QWMOE_ERR_INVALID_ARG;
+    if ((rc = kv_rows(k, k_nb1, n, size)) || (rc = kv_rows(v, v_nb1, n, size))) return rc;
+    a.type = type;
+    a.k_nb1 = k_nb1;
+    a.v_nb1 = v_nb1;
+    a.slot = slot;
+    a.T = T;
+    if ((rc = kv_ready())) return rc;
+    a.status = g_lib.status;
+    return QWMOE_OK;
+}
+
+}  // namespace
+
+size_t qwmoe_kv_q4_page_bytes(int64_t n_head_kv, int64_t n_embd_head, int64_t page_tokens) {
+    if (!kv_shape_ok(n_head_kv, n_embd_head, page_tokens)) return 0;
+    return (size_t) (n_head_kv * (page_tokens / qw::KV_CELL) * 36 * n_embd_head);
+}
+
+int qwmoe_kv_plan(void* stream, const int32_t* held, const int32_t* past, const int32_t* n_new, int64_t n_seq,
+                  int64_t page_tokens, int64_t n_pages, int32_t* page_table, int64_t table_width, int32_t* ring,
+                  const int64_t* counters, int64_t* counters_out, int64_t n_tokens, int32_t* seq_start,
+                  int32_t* seq_len, int64_t* slot, int32_t* pos) {
+    if (!held || !past || !n_new || !page_table || !ring || !counters || !counters_out || !seq_start || !seq_len ||
+        n_seq <= 0 || n_pages <= 0 || table_width <= 0 || n_tokens < 0 || page_tokens <= 0 ||
+        (n_tokens > 0 && (!slot || !pos)) || counters == counters_out)
+        return QWMOE_ERR_INVALID_ARG;
+    const int shift = kv_shift(page_tokens);
+    if (shift < 0 || n_seq > qw::KV_MAX_SEQ || n_pages > 0x7fffffff || n_tokens > 0x7fffffff ||
+        table_width > (0x7fffffff >> shift))
+        return QWMOE_ERR_UNSUPPORTED;
+    if (int rc = kv_ready()) return rc;
+    qw::KvPlanArgs a{};
+    a.held = held;
+    a.past = past;
+    a.n_new = n_new;
+    a.S = (int) n_seq;
+    a.page_shift = shift;
+    a.n_pages = n_pages;
+    a.table = page_table;
+    a.W = table_width;
+    a.ring = ring;
+    a.counters = counters;
+    a.counters_out = counters_out;
+    a.T = n_tokens;
+    a.seq_start = seq_start;
+    a.seq_len = seq_len;
+    a.slot = slot;
+    a.pos = pos;
+    a.status = g_lib.status;
+    return qw::launch_kv_plan(a, S(stream));
+}
+
+int qwmoe_kv_q4_store(void* stream, const qwmoe_kv_q4* cache, int type, const void* k, size_t k_nb1, const void* v,
+                      size_t v_nb1, const int64_t* slot, int64_t n_tokens) {
+    qw::KvRowsArgs a{};
+    if (int rc = kv_rows_args(cache, type, k, k_nb1, v, v_nb1, slot, n_tokens, a)) return rc;
+    a.k = k;
+    a.v = v;
+    return qw::launch_kv_q4_store(a, S(stream));
+}
+
+int qwmoe_kv_q4_load(void* stream, const qwmoe_kv_q4* cache, int type, void* k, size_t k_nb1, void* v, size_t v_nb1,
+                     const int64_t* slot, int64_t n_tokens) {
+    qw::KvRowsArgs a{};
+    if (int rc = kv_rows_args(cache, type, k, k_nb1, v, v_nb1, slot, n_tokens, a)) return rc;
+    a.ko = k;
+    a.vo = v;
+    return qw::launch_kv_q4_load(a, S(stream));
+}
+
+int qwmoe_attn_kv_q4(void* stream, const qwmoe_kv_q4* cache, int type, const void* q, size_t q_nb1, int64_t n_head,
+                     const int32_t* page_table, int64_t table_width, const int32_t* seq_start, const int32_t* seq_len,
+                     int64_t n_seq, int64_t n_tokens, int64_t max_new, int64_t max_len, float kq_scale, void* out,
+                     size_t out_nb1) {
+    qw::AttnQ4Args a{};
+    int rc;
+    if ((rc = kv_cache(cache, a.c))) return rc;
+    const size_t size = kv_type_size(type);
+    if (!size) return QWMOE_ERR_UNSUPPORTED;
+    const int64_t D = cache->n_embd_head;
+    if (!page_table || !seq_start || !seq_len || n_head <= 0 || n_head % cache->n_head_kv || table_width <= 0 ||
+        n_seq <= 0 || n_tokens < 0 || max_new < 0 || max_len < 0 || q == out || !(kq_scale >= 0.0f) ||
+        !(kq_scale < INFINITY))
+        return QWMOE_ERR_INVALID_ARG;
+    if (n_seq > qw::KV_MAX_SEQ || n_head > 65535 || n_tokens > 0x7fffffff / n_head ||
+        table_width > (0x7fffffff >> a.c.page_shift))
+        return QWMOE_ERR_UNSUPPORTED;
+    if (max_len > table_width * cache->page_tokens) return QWMOE_ERR_INVALID_ARG;
+    if ((rc = kv_rows(q, q_nb1, n_head * D, size)) || (rc = kv_rows(out, out_nb1, n_head * D, size))) return rc;
+    if ((rc = kv_ready())) return rc;
+    a.type = type;
+    a.q = q;
+    a.out = out;
+    a.q_nb1 = q_nb1;
+    a.out_nb1 = out_nb1;
+    a.n_head = (int) n_head;
+    a.S = (int) n_seq;
+    a.T = n_tokens;
+    a.W = table_width;
+    a.table = page_table;
+    a.seq_start = seq_start;
+    a.seq_len = seq_len;
+    a.max_new = max_new;
+    a.max_len = max_len;
+    a.scale = (float) ((kq_scale > 0.0f ? (double) kq_scale : 1.0 / sqrt((double) D)) * 1.4426950408889634);
+    a.status = g_lib.status;
+    return qw::launch_attn_q4(a, S(stream));
 }
 
 int qwmoe_ffn_layer(void* stream, const qwmoe_layer* L, const float* x, int64_t T, float* out, float rms_eps,

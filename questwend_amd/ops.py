@@ -11,8 +11,8 @@ import ctypes as C
 import sys
 import weakref
 
-from . import (BLOCK, CACHE_COPY_ENGINE, CACHE_DRY_RUN, Q8_0, Q8_K, ExpertCacheConfig, ExpertCacheStats, ExpertSrc, GgufTensorInfo, Layer, SharedExpert,
-               MoeHparams, check, lib, row_size, vec_dot_type)
+from . import (BF16, BLOCK, CACHE_COPY_ENGINE, CACHE_DRY_RUN, F16, F32, Q8_0, Q8_K, ExpertCacheConfig, ExpertCacheStats,
+               ExpertSrc, GgufTensorInfo, KvQ4, Layer, MoeHparams, SharedExpert, check, lib, row_size, vec_dot_type)
 
 
 def _torch():
@@ -471,6 +471,131 @@ def decoder_layer(attn, moe: Layer, h, n_past: int, rms_eps: float = 1e-6):
     check(lib().qwmoe_decoder_layer(stream(), C.byref(attn), C.byref(moe), _ptr(h), T, n_past, rms_eps, _ptr(out),
                                     _ptr(ids), _ptr(w)), "decoder_layer")
     return out, ids, w
+
+
+def _kv_type(dtype) -> int:
+    torch = _torch()
+    t = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
+    if t is None:
+        raise TypeError(f"rows of {dtype}: the cache takes float32, float16 and bfloat16")
+    return t
+
+
+def _kv_rows(x, name: str, heads: int, D: int):
+    """Byte stride between the token rows of x [T, heads, D]; the heads of a token are dense."""
+    if x.dim() != 3 or tuple(x.shape[1:]) != (heads, D):
+        raise ValueError(f"{name}: [tokens, {heads}, {D}] is wanted, got {tuple(x.shape)}")
+    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != D):
+        raise ValueError(f"{name}: the heads of a token have to be dense")
+    return x.stride(0) * x.element_size() if x.shape[0] > 1 else heads * D * x.element_size()
+
+
+def _kv_index(x, name: str, dtype, *shape):
+    if x.dtype != dtype or not x.is_contiguous() or any(n is not None and m != n for m, n in zip(x.shape, shape)) \
+            or x.dim() != len(shape):
+        raise ValueError(f"{name}: dense {dtype} {shape} is wanted, got {x.dtype} {tuple(x.shape)}")
+
+
+def kv_q4_page_bytes(n_head_kv: int, D: int, page_tokens: int) -> int:
+    """Bytes of a page of the 4-bit cache (0: a shape it does not take)."""
+    return int(lib().qwmoe_kv_q4_page_bytes(n_head_kv, D, page_tokens))
+
+
+def make_kv_q4(data, n_head_kv: int, D: int, page_tokens: int = 64) -> KvQ4:
+    """A ``qwmoe_kv_q4`` over ``data``, a dense uint8 tensor of whole pages (it is kept alive)."""
+    size = kv_q4_page_bytes(n_head_kv, D, page_tokens)
+    if not size:
+        raise ValueError(f"{n_head_kv} heads of {D}, pages of {page_tokens}: not a shape of the 4-bit cache")
+    if data.dtype != _torch().uint8 or not data.is_contiguous() or data.numel() < size or data.numel() % size:
+        raise ValueError(f"data: dense uint8 pages of {size} bytes are wanted")
+    c = KvQ4(n_head_kv, D, page_tokens, data.numel() // size, data.data_ptr())
+    c.keep = data
+    return c
+
+
+def kv_plan(held, past, new, page_tokens: int, page_table, ring, counters, n_tokens: int):
+    """One round of bookkeeping (qwmoe_kv_plan): held, past, new i32 [S]; page_table i32
+    [S, W] and ring i32 [n_pages] are updated in place; counters i64 [2] (head, tail).
+    Returns (the next counters, seq_start [S + 1], seq_len [S], slot i64 [n_tokens], pos [n_tokens])."""
+    torch = _torch()
+    S, W = page_table.shape
+    for x, name in ((held, "held"), (past, "past"), (new, "new")):
+        _kv_index(x, name, torch.int32, S)
+    _kv_index(page_table, "page_table", torch.int32, S, W)
+    _kv_index(ring, "ring", torch.int32, None)
+    _kv_index(counters, "counters", torch.int64, 2)
+    dev = held.device
+    out = torch.empty(2, dtype=torch.int64, device=dev)
+    start = torch.empty(S + 1, dtype=torch.int32, device=dev)
+    length = torch.empty(S, dtype=torch.int32, device=dev)
+    slot = torch.empty(n_tokens, dtype=torch.int64, device=dev)
+    pos = torch.empty(n_tokens, dtype=torch.int32, device=dev)
+    check(lib().qwmoe_kv_plan(stream(), _ptr(held), _ptr(past), _ptr(new), S, page_tokens, ring.numel(), _ptr(page_table), W,
+                              _ptr(ring), _ptr(counters), _ptr(out), n_tokens, _ptr(start), _ptr(length), _ptr(slot),
+                              _ptr(pos)), "kv_plan")
+    return out, start, length, slot, pos
+
+
+def kv_q4_store(cache: KvQ4, k, v, slot) -> None:
+    """k, v [T, n_head_kv, D] (f32, f16 or bf16; token rows may be strided) quantized into the
+    cache at slot i64 [T] (negative: passed over)."""
+    torch = _torch()
+    T = k.shape[0]
+    nbk = _kv_rows(k, "k", cache.n_head_kv, cache.n_embd_head)
+    nbv = _kv_rows(v, "v", cache.n_head_kv, cache.n_embd_head)
+    if v.dtype != k.dtype or v.shape[0] != T:
+        raise ValueError("k and v: one type and one number of rows are wanted")
+    _kv_index(slot, "slot", torch.int64, T)
+    typ = _kv_type(k.dtype)
+    if T:
+        check(lib().qwmoe_kv_q4_store(stream(), C.byref(cache), typ, _ptr(k), nbk, _ptr(v), nbv, _ptr(slot), T),
+              "kv_q4_store")
+
+
+def kv_q4_load(cache: KvQ4, slot, dtype=None, out=None):
+    """The cache's rows at slot i64 [T]: (k, v) [T, n_head_kv, D] of ``dtype`` (f32), or into
+    out = (k, v).  Rows with a negative slot are not written."""
+    torch = _torch()
+    T = slot.shape[0]
+    if out is None:
+        shape = (T, cache.n_head_kv, cache.n_embd_head)
+        out = tuple(torch.empty(shape, dtype=dtype or torch.float32, device=slot.device) for _ in range(2))
+    k, v = out
+    nbk = _kv_rows(k, "k", cache.n_head_kv, cache.n_embd_head)
+    nbv = _kv_rows(v, "v", cache.n_head_kv, cache.n_embd_head)
+    if v.dtype != k.dtype or k.shape[0] != T or v.shape[0] != T:
+        raise ValueError("k and v: one type and a row per slot are wanted")
+    _kv_index(slot, "slot", torch.int64, T)
+    typ = _kv_type(k.dtype)
+    if T:
+        check(lib().qwmoe_kv_q4_load(stream(), C.byref(cache), typ, _ptr(k), nbk, _ptr(v), nbv, _ptr(slot), T),
+              "kv_q4_load")
+    return k, v
+
+
+def attn_kv_q4(cache: KvQ4, q, page_table, seq_start, seq_len, max_new: int, max_len: int, scale: float = 0.0, out=None):
+    """Causal attention of a batch over the 4-bit cache (qwmoe_attn_kv_q4).  q [T, n_head, D]
+    (f32, f16 or bf16; token rows may be strided), page_table i32 [S, W], seq_start i32
+    [S + 1], seq_len i32 [S]; max_new, max_len bound the requests' new tokens and
+    lengths; scale 0: 1 / sqrt(D).  Returns out; rows behind the last request are not written."""
+    torch = _torch()
+    T, nq, D = q.shape
+    S, W = page_table.shape
+    nbq = _kv_rows(q, "q", nq, cache.n_embd_head)
+    if out is None:
+        out = torch.empty((T, nq, D), dtype=q.dtype, device=q.device)
+    nbo = _kv_rows(out, "out", nq, D)
+    if out.dtype != q.dtype or out.shape[0] != T:
+        raise ValueError("out: q's type and number of rows are wanted")
+    _kv_index(page_table, "page_table", torch.int32, S, W)
+    _kv_index(seq_start, "seq_start", torch.int32, S + 1)
+    _kv_index(seq_len, "seq_len", torch.int32, S)
+    typ = _kv_type(q.dtype)
+    if T:
+        check(lib().qwmoe_attn_kv_q4(stream(), C.byref(cache), typ, _ptr(q), nbq, nq, _ptr(page_table), W,
+                                     _ptr(seq_start), _ptr(seq_len), S, T, max_new, max_len, scale, _ptr(out), nbo),
+              "attn_kv_q4")
+    return out
 
 
 class Gguf(_Handle):
