@@ -1129,6 +1129,20 @@ int qwmoe_attn_kv_q4(void* stream, const qwmoe_kv_q4* cache, int type, const voi
     a.max_len = max_len;
     a.scale = (float) ((kq_scale > 0.0f ? (double) kq_scale : 1.0 / sqrt((double) D)) * 1.4426950408889634);
     a.status = g_lib.status;
+    if (n_tokens == 0) return QWMOE_OK;
+    // as many splits of the keys as fill the card and as the workspace holds
+    Arena ar(kReserved);
+    const size_t per = (size_t) (n_tokens * n_head) * (size_t) (D + 2) * 4, room = ar.left();
+    int64_t splits = std::min<int64_t>(qw::q4_splits(a), room > 1024 ? (int64_t) ((room - 1024) / per) : 0);
+    const int64_t cells = std::max<int64_t>((max_len + qw::KV_CELL - 1) / qw::KV_CELL, 1);
+    if (splits < 2) splits = 1;
+    a.cells = (cells + splits - 1) / splits;
+    a.splits = (int) ((cells + a.cells - 1) / a.cells);
+    if (a.splits > 1) {
+        a.part = ar.take<float>((size_t) (a.splits * n_tokens * n_head * D));
+        a.stat = ar.take<float>((size_t) (a.splits * n_tokens * n_head * 2));
+        if (!a.part || !a.stat) return QWMOE_ERR_WORKSPACE;
+    }
     return qw::launch_attn_q4(a, S(stream));
 }
 

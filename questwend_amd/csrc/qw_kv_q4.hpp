@@ -81,8 +81,15 @@ struct AttnQ4Args {
     const int32_t *table, *seq_start, *seq_len;
     int64_t max_new, max_len;
     float scale;                          // of the scores, times log2(e)
+    int64_t cells;                        // cells of 32 keys per split
+    int splits;
+    float *part, *stat;                   // [splits][T][n_head][D] sums and [..][2] offset, sum of weights (splits > 1)
     int32_t* status;
 };
+// Tiles of 16 columns per wave, blocks of `per` rows, and how many splits of the keys fill the card.
+int q4_tiles(const AttnQ4Args& a);
+int64_t q4_blocks(const AttnQ4Args& a, int per);
+int64_t q4_splits(const AttnQ4Args& a);
 int launch_attn_q4(const AttnQ4Args& a, hipStream_t stream);
 
 }  // namespace qw
