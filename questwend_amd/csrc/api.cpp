@@ -1132,17 +1132,22 @@ int qwmoe_attn_kv_q4(void* stream, const qwmoe_kv_q4* cache, int type, const voi
     if (n_tokens == 0) return QWMOE_OK;
     // as many splits of the keys as fill the card and as the workspace holds
     Arena ar(kReserved);
-    const size_t per = (size_t) (n_tokens * n_head) * (size_t) (D + 2) * 4, room = ar.left();
-    int64_t splits = std::min<int64_t>(qw::q4_splits(a), room > 1024 ? (int64_t) ((room - 1024) / per) : 0);
     const int64_t cells = std::max<int64_t>((max_len + qw::KV_CELL - 1) / qw::KV_CELL, 1);
-    if (splits < 2) splits = 1;
-    a.cells = (cells + splits - 1) / splits;
-    a.splits = (int) ((cells + a.cells - 1) / a.cells);
-    if (a.splits > 1) {
-        a.part = ar.take<float>((size_t) (a.splits * n_tokens * n_head * D));
-        a.stat = ar.take<float>((size_t) (a.splits * n_tokens * n_head * 2));
-        if (!a.part || !a.stat) return QWMOE_ERR_WORKSPACE;
-    }
+    a.tcap = qw::q4_few_tokens(a);
+    auto split = [&](int64_t want, int64_t rows, int64_t& per, int& n, float*& part, float*& stat) {
+        const size_t bytes = (size_t) (rows * (D + 2)) * 4, room = ar.left();
+        const int64_t fit = room > 2048 ? (int64_t) ((room - 2048) / std::max<size_t>(bytes, 1)) : 0;
+        const int64_t k = std::min(want, fit) < 2 ? 1 : std::min(want, fit);
+        per = (cells + k - 1) / k;
+        n = (int) ((cells + per - 1) / per);
+        if (n == 1) return true;
+        part = ar.take<float>((size_t) (n * rows * D));
+        stat = ar.take<float>((size_t) (n * rows * 2));
+        return part && stat;
+    };
+    if (!split(qw::q4_splits(a), a.S * a.tcap * n_head, a.cells, a.splits, a.part, a.stat) ||
+        !split(qw::q4_row_splits(a), n_tokens * n_head, a.row_cells, a.row_splits, a.row_part, a.row_stat))
+        return QWMOE_ERR_WORKSPACE;
     return qw::launch_attn_q4(a, S(stream));
 }
 

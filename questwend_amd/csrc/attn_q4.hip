@@ -28,10 +28,10 @@
 // the value scales when it was last set, and it is set anew when some weight passes 2^12
 // or some scale 2^E.  Otherwise a cell costs no exchange between lanes and no rescaling.
 //
-// A workgroup of four waves takes a block of a request's rows (R = n_head / n_head_kv rows
-// per token) of one kv head and one split of the keys; each wave NC tiles of the rows, or,
-// where the block has rows for one wave only, a quarter of the cells (their sums meet in
-// LDS).  The next cell's dwords are loaded while this one's are computed on.
+// A workgroup takes a request's rows (R = n_head / n_head_kv per token), one kv head and one
+// split of the keys.  Its waves share out 16-column tiles of the rows, and waves of the
+// same tile share out the cells; their sums meet in LDS, the splits' in a second launch.
+// The next cell's dwords are loaded while this one's are computed on.
 #include <algorithm>
 #include <type_traits>
 
@@ -60,78 +60,86 @@ __device__ __forceinline__ void q4_put4(void* p, int type, int64_t i, f4 v) {
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The request that holds a block of rows (`per` rows a block, R rows per token): request
-// i's blocks are numbered from floor(seq_start[i] R / per) + i on, which leaves room for
-// every one of its blocks whatever the lengths, and is known without a prefix sum.
+// A request as the call gives it.
 struct Q4Seq {
     int i, n, len;     // request, its new tokens, its keys (0: rows of zeros)
-    int64_t row0;      // its first token row
+    int row0;          // its first token row
 };
-__device__ __forceinline__ int64_t q4_block0(const AttnQ4Args& a, int i, int R, int per) {
-    const int64_t t = min(max((int64_t) a.seq_start[i], (int64_t) 0), a.T);
-    return t * R / per + i;
+__device__ __forceinline__ bool q4_request(const AttnQ4Args& a, int i, Q4Seq& s) {
+    s.i = i;
+    s.row0 = a.seq_start[i];
+    const int64_t end = a.seq_start[i + 1];
+    s.len = a.seq_len[i];
+    s.n = (int) (end - s.row0);
+    return s.row0 >= 0 && end > s.row0 && end <= a.T;
 }
-// The last of 0 .. n - 1 that `ok` holds for (it holds up to some place and not beyond), -1:
-// none.  Called by whole waves, 64 candidates at a time.
+// The last request whose key(first token row, number) is at most `want` (keys ascend).  Called
+// by whole waves: 64 candidates at a time, whose rows and lengths come with the same loads.
 template <typename F>
-__device__ __forceinline__ int q4_last(int n, int lane, F ok) {
-    int lo = 0, step = (n + 63) / 64;
+__device__ __forceinline__ bool q4_find(const AttnQ4Args& a, int lane, int64_t want, F key, Q4Seq& s) {
+    int lo = 0, step = (a.S + 63) / 64;
     for (;;) {
-        const int i = lo + lane * step;
-        const uint64_t m = __ballot(i < n && ok(min(i, n - 1)));
-        if (m == 0) return -1;
-        lo = uni(lo + (__popcll(m) - 1) * step);
-        if (step == 1) return lo;
+        const int i = min(lo + lane * step, a.S - 1);
+        const int t0 = a.seq_start[i], t1 = a.seq_start[i + 1], len = a.seq_len[i];
+        const uint64_t m = __ballot(lo + lane * step < a.S && key(t0, i) <= want);
+        if (m == 0) return false;
+        const int at = 63 - __builtin_clzll(m);
+        lo += at * step;
+        if (step == 1) {
+            s.i = uni(lo);
+            s.row0 = __builtin_amdgcn_readlane(t0, at);
+            const int64_t end = __builtin_amdgcn_readlane(t1, at);
+            s.n = (int) (end - s.row0);
+            s.len = __builtin_amdgcn_readlane(len, at);
+            return s.row0 >= 0 && end > s.row0 && end <= a.T;
+        }
         step = (step + 63) / 64;
     }
-}
-__device__ __forceinline__ bool q4_request(const AttnQ4Args& a, int i, Q4Seq& s) {
-    if (i < 0) return false;
-    const int64_t t0 = a.seq_start[i], t1 = a.seq_start[i + 1];
-    s.i = i;
-    s.row0 = t0;
-    if (t0 < 0 || t1 > a.T || t1 <= t0) return false;
-    s.n = (int) (t1 - t0);
-    s.len = a.seq_len[i];
-    return true;
 }
 // Whether the request's lengths fit the call.
 __device__ __forceinline__ bool q4_fits(const AttnQ4Args& a, const Q4Seq& s) {
     return s.len >= 0 && s.len <= a.max_len && s.n <= a.max_new;
 }
 
-// One cell's dwords as they lie in memory.
+// One cell's dwords as they lie in memory: keys, values.
 template <int D>
-struct Q4Cell {
+struct Q4Keys {
     static constexpr int NB = D / 32;
-    uint32_t k[2][NB];          // key codes of token l % 16 of both halves, dims 8 (l / 16) .. of each block
-    uint32_t v[NB][2];          // value codes of dims l % 16 and 16 + l % 16 of each block, keys 4 (l / 16) ..
-    uint32_t ks[2][NB][2];      // scales of keys 4 (l / 16) .. + 3 of both halves
-    uint32_t vs[2][NB][2];
-    uint32_t chk[(NB + 3) / 4]; // the lane's share of the value scales (NB / 2 halves)
-
+    uint32_t c[2][NB];       // codes of token l % 16 of both halves, dims 8 (l / 16) .. of each block
+    uint32_t d[2][NB][2];    // scales of keys 4 (l / 16) .. + 3 of both halves
     __device__ __forceinline__ void load(const uint8_t* cell, int l) {
         const int m = l & 15, g = l >> 4;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) __builtin_memcpy(k[u], cell + (uint32_t) (((16 * u + m) * 4 + g) * NB * 4), 4 * NB);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) __builtin_memcpy(ks[u], cell + (uint32_t) (16 * D + (4 * u + g) * NB * 8), 8 * NB);
+        for (int u = 0; u < 2; ++u) {
+            __builtin_memcpy(c[u], cell + (uint32_t) (((16 * u + m) * 4 + g) * NB * 4), 4 * NB);
+            __builtin_memcpy(d[u], cell + (uint32_t) (16 * D + (4 * u + g) * NB * 8), 8 * NB);
+        }
+    }
+};
+template <int D>
+struct Q4Values {
+    static constexpr int NB = D / 32;
+    uint32_t c[NB][2];           // codes of dims l % 16 and 16 + l % 16 of each block, keys 4 (l / 16) .. of both halves
+    uint32_t d[2][NB][2];        // scales of the same keys
+    uint32_t chk[(NB + 3) / 4];  // the lane's share of the scales (NB / 2 halves)
+    __device__ __forceinline__ void load(const uint8_t* cell, int l) {
+        const int m = l & 15, g = l >> 4;
 #pragma unroll
         for (int b = 0; b < NB; b += 2)
-            __builtin_memcpy(v[b], cell + (uint32_t) (18 * D + (((b / 2) * 16 + m) * 4 + g) * 16), 16);
+            __builtin_memcpy(c[b], cell + (uint32_t) (18 * D + (((b / 2) * 16 + m) * 4 + g) * 16), 16);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) __builtin_memcpy(vs[u], cell + (uint32_t) (34 * D + (4 * u + g) * NB * 8), 8 * NB);
+        for (int u = 0; u < 2; ++u) __builtin_memcpy(d[u], cell + (uint32_t) (34 * D + (4 * u + g) * NB * 8), 8 * NB);
         if constexpr (NB == 2) chk[0] = *(const uint16_t*) (cell + (uint32_t) (34 * D + 2 * l));
         else __builtin_memcpy(chk, cell + (uint32_t) (34 * D + NB * l), NB);
     }
-    // the largest magnitude among the lane's halves of keys below `keys`, as f16 bits; NaNs count as 0
-    __device__ __forceinline__ uint32_t top(int l, int keys, bool all) const {
+    // the largest magnitude among the lane's share, of keys below `keys`, as f16 bits; NaNs count as 0
+    __device__ __forceinline__ uint32_t top(int l, int keys) const {
         uint32_t t = 0;
 #pragma unroll
         for (int e = 0; e < NB / 2; ++e) {
             uint32_t x = (chk[e / 2] >> (16 * (e & 1))) & 0x7fffu;
             const int at = l * (NB / 2) + e, key = 4 * (at / (4 * NB)) + at % 4;
-            x = x > 0x7c00u || (!all && key >= keys) ? 0u : x;
+            x = x > 0x7c00u || key >= keys ? 0u : x;
             t = max(t, x);
         }
         return t;
@@ -170,116 +178,99 @@ __device__ __forceinline__ uint32_t codes(uint32_t w) {
 // (lane l ^ 8 of the same 16)
 __device__ __forceinline__ float other_part(float v) { return dpp_f<0x128>(v); }   // row_ror:8
 
-// NS f16 parts per row (f32 rows: two), NC tiles of 16 / NS rows per wave.
-template <int D, int NS, int NC>
-__global__ void __launch_bounds__(256) k_attn_q4(AttnQ4Args a) {
-    constexpr int NB = D / 32, RC = 16 / NS, RW = NC * RC;
+// Waves of a workgroup, and per SIMD, that the registers leave room for; two cells' dwords in flight
+// where they fit.
+constexpr int q4_group(int D) { return D == 256 ? 4 : 8; }
+constexpr int q4_simd(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }
+constexpr int q4_buffers(int D) { return D <= 128 ? 2 : 1; }
+
+// A row's q (NS f16 parts; lane l has dims 8 (l / 16) .. of each block, f32 rows' low parts in
+// columns 8 .. 15), scaled by a power of two into f16's upper range; returns the scores'
+// factor: scale log2(e) over that power.
+template <int D, int NS>
+__device__ __forceinline__ float q4_load_q(const AttnQ4Args& a, int tok, int h, bool ok, int l, h8 (&q)[D / 32]) {
+    constexpr int NB = D / 32;
+    float x[NB][8];
+    const char* src = (const char*) a.q + (int64_t) tok * a.q_nb1;
+    const int at = h * D + 8 * (l >> 4);
+    if constexpr (NS == 2) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const f4 lo = *(const f4*) ((const float*) src + at + 32 * b), hi = *(const f4*) ((const float*) src + at + 32 * b + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[b][j] = j < 4 ? lo[j & 3] : hi[j & 3];
+        }
+    } else {
+        const bool f16 = a.type == KV_F16;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const u32x4 v = *(const u32x4*) ((const uint16_t*) src + at + 32 * b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t word = v[j / 2];
+                x[b][j] = f16 ? half_of(word, j & 1) : bitsf(j & 1 ? word & 0xffff0000u : word << 16);
+            }
+        }
+    }
+    float big = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, __builtin_fabsf(x[b][j]));
+    big = fmaxf(big, __shfl_xor(big, 16));
+    big = fmaxf(big, __shfl_xor(big, 32));
+    // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
+    const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
+    const float up = ok ? bitsf((uint32_t) (127 + 14 - ex) << 23) : 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = x[b][j] * up;
+            const _Float16 v = (_Float16) y;
+            q[b][j] = NS == 2 && (l & 15) >= 8 ? (_Float16) (y - (float) v) : v;
+        }
+    return a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
+}
+
+// NS f16 parts per row (f32 rows: two).
+template <int D, int NS>
+__global__ void __launch_bounds__(64 * q4_group(D)) __attribute__((amdgpu_waves_per_eu(q4_simd(D), q4_simd(D)))) k_attn_q4(AttnQ4Args a) {
+    constexpr int NB = D / 32, RC = 16 / NS, W = q4_group(D), BUF = q4_buffers(D);
     constexpr int LD = D + 4;                                   // floats of a row in LDS
-    __shared__ __align__(16) float s_o[4 * RC * LD];
-    __shared__ float s_off[4][NC * RC], s_l[4][NC * RC];
+    __shared__ __align__(16) float s_o[W * RC * LD];
+    __shared__ float s_off[W][RC], s_l[W][RC];
     const int tid = threadIdx.x, l = tid & 63, m = l & 15, g = l >> 4;
     const int w = uni(tid >> 6);
-    const int R = a.n_head / a.c.n_head_kv, hd = blockIdx.y, z = blockIdx.z;
+    const unsigned R = (unsigned) a.n_head / (unsigned) a.c.n_head_kv;
+    const int hd = blockIdx.y, z = blockIdx.z;
     Q4Seq s;
-    if (!q4_request(a, q4_last(a.S, l, [&](int i) { return q4_block0(a, i, R, 4 * RW) <= blockIdx.x; }), s)) return;
-    const int64_t rows = (int64_t) s.n * R, base = ((int64_t) blockIdx.x - q4_block0(a, s.i, R, 4 * RW)) * (4 * RW);
-    if (base >= rows) return;
+    if (!q4_request(a, blockIdx.x, s)) return;
+    const int rows = (int) min((int64_t) s.n * R, (int64_t) 1 << 30);
+    if (rows > W * RC) return;                                  // (k_attn_q4_rows')
     int len = s.len;
     if (!q4_fits(a, s)) {
         len = 0;
         if (tid == 0) atomicOr(a.status, QWMOE_STATUS_BAD_SEQ);
     }
-    const bool share = rows - base <= RW;                       // rows for one wave only: its cells go to all four
-    const int64_t r0 = base + (share ? 0 : w * RW);             // the wave's first row
-    const int wrows = (int) max(min(rows - r0, (int64_t) RW), (int64_t) 0);
-    const int wtiles = (wrows + RC - 1) / RC;
+    // the waves of the workgroup: 2^tshift tiles of rows, 2^cshift waves each
+    const int tshift = rows <= RC ? 0 : rows <= 2 * RC ? 1 : rows <= 4 * RC ? 2 : 3;
+    const int cshift = (W == 8 ? 3 : 2) - tshift;
+    const int r0 = (w & ((1 << tshift) - 1)) * RC;              // the wave's first row
+    const int wrows = max(min(rows - r0, RC), 0);
     const int back = len - s.n;                                 // a row of token t sees keys .. back + t
-    const int last = wrows ? back + (int) ((r0 + wrows - 1) / R) : -1;   // the last key some row of the wave sees
-    const int every = back + (int) (r0 / R);                    // keys up to here are seen by all of its rows
+    const int last = wrows ? back + (int) ((unsigned) (r0 + wrows - 1) / R) : -1;   // the last key some row of the wave sees
+    const int every = back + (int) ((unsigned) r0 / R);         // keys up to here are seen by all of its rows
     const int cells = last < 0 ? 0 : (last >> 5) + 1;
-    const int cshift = share ? 2 : 0;                           // the wave's cells: c0, c0 + 2^cshift ..
-    const int c0 = (int) min((int64_t) z * a.cells + (share ? w : 0), (int64_t) cells);
-    const int c1 = (int) min((int64_t) (z + 1) * a.cells, (int64_t) cells);
-    const int block_last = back + (int) ((min(rows, base + 4 * RW) - 1) / R);
-    if (z > 0 && (int64_t) z * a.cells > (block_last >> 5)) return;   // (z = 0 writes the rows without keys)
+    const int zc = (int) min((int64_t) z * a.cells, (int64_t) 1 << 30);
+    if (z > 0 && zc > (len - 1) >> 5) return;                   // (z = 0 writes the rows without keys)
+    const int c0 = min(zc + (w >> tshift), cells);              // its cells: c0, c0 + 2^cshift ..
+    const int c1 = (int) min(zc + a.cells, (int64_t) cells);
 
-    // this lane's rows
-    int lim[NC];            // the last key its row sees
-    h8 q[NC][NB];
-    float qs[NC];           // the scores' factor: scale log2(e), 2^9 for the codes, q's power of two
-    int64_t orow[NC];       // token row * n_head + head, -1 without one
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const bool ok = n * RC + (m % RC) < wrows;
-        const int64_t r = ok ? r0 + n * RC + (m % RC) : 0;
-        const int t = (int) (r / R), h = hd * R + (int) (r % R);
-        orow[n] = ok ? (s.row0 + t) * a.n_head + h : -1;
-        lim[n] = ok ? back + t : -1;
-        float x[NB][8];
-        const char* src = (const char*) a.q + (s.row0 + t) * a.q_nb1;
-        const int64_t at = (int64_t) h * D + 8 * g;
-        if constexpr (NS == 2) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const f4 lo = *(const f4*) ((const float*) src + at + 32 * b), hi = *(const f4*) ((const float*) src + at + 32 * b + 4);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[b][j] = j < 4 ? lo[j & 3] : hi[j & 3];
-            }
-        } else {
-            const bool f16 = a.type == KV_F16;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const u32x4 v = *(const u32x4*) ((const uint16_t*) src + at + 32 * b);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t word = v[j / 2];
-                    x[b][j] = f16 ? half_of(word, j & 1) : bitsf(j & 1 ? word & 0xffff0000u : word << 16);
-                }
-            }
-        }
-        float big = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[b][j] = ok ? x[b][j] : 0.0f;
-                big = fmaxf(big, __builtin_fabsf(x[b][j]));
-            }
-        big = fmaxf(big, __shfl_xor(big, 16));
-        big = fmaxf(big, __shfl_xor(big, 32));
-        // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex) lies in f16's upper range
-        const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
-        const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
-        qs[n] = a.scale * bitsf((uint32_t) (127 - 5 + ex) << 23);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            h8 part;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = x[b][j] * up;
-                _Float16 v = (_Float16) y;
-                if (NS == 2 && m >= RC) v = (_Float16) (y - (float) v);
-                part[j] = v;
-            }
-            q[n][b] = part;
-        }
-    }
-
-    f4 o[NC][2 * NB];            // O^T 2^-9: dims 16 tile + 4 g + i of the lane's row
-    float off[NC], mx[NC], lsum[NC];
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        off[n] = mx[n] = NO_KEY;
-        lsum[n] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) o[n][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    int E = -25;                 // the value scales so far are at most 2^E
-    uint32_t Ebits = 0;          // 2^E as f16 bits
-
+    // cells: their pages, 64 of the wave's at a time, one per lane
     const int32_t* pages = a.table + (int64_t) s.i * a.W;
     const int cpp = a.c.page_shift - 5;                         // log2 of a page's cells
-    int pg = 0, pg_at = c0;                                     // the pages of 64 of the wave's cells, one per lane
+    int pg = 0, pg_at = c0;
     auto fetch_pages = [&](int c) {
         pg_at = c;
         const int mine = c + (l << cshift);
@@ -290,51 +281,77 @@ __global__ void __launch_bounds__(256) k_attn_q4(AttnQ4Args a) {
         }
     };
     auto page_of = [&](int c) { return __builtin_amdgcn_readlane(pg, (c - pg_at) >> cshift); };
-    auto address = [&](int c, int page) {
-        return a.c.data + (int64_t) max(page, 0) * a.c.page_bytes() + hd * a.c.head_bytes() +
-               (int64_t) (c & ((1 << cpp) - 1)) * (36 * D);
-    };
+    const uint8_t* head = a.c.data + hd * a.c.head_bytes();
+    const int64_t page_bytes = a.c.page_bytes();
+    auto address = [&](int c, int page) { return head + max(page, 0) * page_bytes + (c & ((1 << cpp) - 1)) * (36 * D); };
+    Q4Keys<D> xk[BUF];
+    Q4Values<D> xv[BUF];
+    int c = c0, page = 0;
+    if (c < c1) {
+        fetch_pages(c);
+        page = page_of(c);
+        const uint8_t* cell = address(c, page);
+        xk[0].load(cell, l);
+        xv[0].load(cell, l);
+    }
 
-    auto step = [&](const Q4Cell<D>& x, int c, bool gone, auto masked) __attribute__((always_inline)) {
-        constexpr bool MASK = decltype(masked)::value;          // some row does not see some key of the cell
-        f4 sc[NC][2];
+    // this lane's row
+    const int r = r0 + (m & (RC - 1));
+    const bool ok = r < rows;
+    const int t = ok ? (int) ((unsigned) r / R) : 0, h = ok ? hd * (int) R + (int) ((unsigned) r % R) : 0;
+    const int lim = ok ? back + t : -1;                         // the last key it sees
+    h8 q[NB];
+    const float qs = 512.0f * q4_load_q<D, NS>(a, s.row0 + t, h, ok, l, q);
+
+    f4 o[2 * NB];                // O^T 2^-9: dims 16 tile + 4 g + i of the lane's row
 #pragma unroll
-        for (int n = 0; n < NC; ++n) sc[n][0] = sc[n][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < 2 * NB; ++i) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float off = NO_KEY, mx = NO_KEY, lsum = 0.0f;
+    int E = -25;                 // the value scales so far are at most 2^E
+    uint32_t Ebits = 0;          // 2^E as f16 bits
+
+    // one cell; with two buffers the next one's loads go out first, with one buffer its keys' when these
+    // are used and its values' likewise
+    auto turn = [&](int now) __attribute__((always_inline)) {
+        Q4Keys<D>&ck = xk[now % BUF], &nk = xk[(now + 1) % BUF];
+        Q4Values<D>&cv = xv[now % BUF], &nv = xv[(now + 1) % BUF];
+        const int next = c + (1 << cshift);
+        const uint8_t* cell = nullptr;
+        const bool gone = page < 0;
+        if (next < c1) {
+            if ((next - pg_at) >> cshift >= 64) fetch_pages(next);
+            page = page_of(next);
+            cell = address(next, page);
+            if (BUF == 2) {
+                nk.load(cell, l);
+                nv.load(cell, l);
+            }
+        }
+        const bool masked = 32 * c + 31 > every || gone;        // some row does not see some key of the cell
+        const int key0 = 32 * c + 4 * g, see = gone ? -1 : lim; // key i of half u: key0 + 16 u + i
+        f4 sc[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const uint32_t c4 = x.k[u][b], d4 = c4 >> 8;
+                const uint32_t c4 = ck.c[u][b], d4 = c4 >> 8;
                 const h8 ka = as_h8(codes<0>(c4), codes<1>(c4), codes<0>(d4), codes<1>(d4));
+                const f4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int n = 0; n < NC; ++n) {
-                    if (n && n >= wtiles) continue;   // uniform
-                    const f4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[n][b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sc[n][u][i] = __builtin_fmaf(p[i], half_of(x.ks[u][b][i / 2], i & 1), sc[n][u][i]);
-                }
+                for (int i = 0; i < 4; ++i) sc[u][i] = __builtin_fmaf(p[i], half_of(ck.d[u][b][i / 2], i & 1), sc[u][i]);
             }
-        const uint32_t top = x.top(l, last + 1 - 32 * c, !MASK);
-        bool move = top > Ebits;
-        const float most = 12.0f - (float) E;
+        if (BUF == 1 && next < c1) nk.load(cell, l);
+        if (NS == 2)
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            if (n && n >= wtiles) continue;
-            float smax = -INFINITY;
+            for (int i = 0; i < 8; ++i) sc[i / 4][i % 4] += other_part(sc[i / 4][i % 4]);
+        if (masked)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int i = 0; i < 8; ++i) sc[i / 4][i % 4] = key0 + 16 * (i / 4) + i % 4 <= see ? sc[i / 4][i % 4] : -INFINITY;
+        float smax = sc[0][0];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = sc[n][u][i];
-                    if (NS == 2) v += other_part(v);
-                    if (MASK) v = !gone && 32 * c + 16 * u + 4 * g + i <= lim[n] ? v : -INFINITY;
-                    sc[n][u][i] = v;
-                    smax = fmaxf(smax, v);
-                }
-            move |= __builtin_fmaf(smax, qs[n], -off[n]) > most;
-        }
-        if (__any(move)) {
+        for (int i = 1; i < 8; ++i) smax = fmaxf(smax, sc[i / 4][i % 4]);
+        const uint32_t top = cv.top(l, last + 1 - 32 * c);
+        if (__any(top > Ebits || __builtin_fmaf(smax, qs, -off) > 12.0f - (float) E)) {
             uint32_t t = top;
 #pragma unroll
             for (int k = 32; k >= 1; k >>= 1) t = max(t, (uint32_t) __shfl_xor((int) t, k));
@@ -343,170 +360,487 @@ __global__ void __launch_bounds__(256) k_attn_q4(AttnQ4Args a) {
                 E = max((int) (t >> 10), 1) - 14;
                 Ebits = (uint32_t) (E + 15) << 10;
             }
+            smax = fmaxf(smax, __shfl_xor(smax, 16));
+            smax = fmaxf(smax, __shfl_xor(smax, 32));
+            mx = fmaxf(mx, smax * qs);
+            const float now_off = mx == NO_KEY ? NO_KEY : mx + (float) (E - 4);
+            const float f = exp2_hw(off - now_off);
+            off = now_off;
+            lsum *= f;
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                if (n && n >= wtiles) continue;
-                float smax = -INFINITY;
+            for (int i = 0; i < 2 * NB; ++i) o[i] *= f;
+        }
+        // weights, formed in place
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+        for (int i = 0; i < 8; ++i) {
+            const float p = exp2_hw(__builtin_fmaf(sc[i / 4][i % 4], qs, -off));
+            sc[i / 4][i % 4] = p;
+            lsum += p;
+        }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) smax = fmaxf(smax, sc[n][u][i]);
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t x0 = cv.c[b][0], x1 = cv.c[b][1], y0 = x0 >> 8, y1 = x1 >> 8;
+            const h8 va[2] = {as_h8(codes<0>(x0), codes<0>(y0), codes<0>(x1), codes<0>(y1)),
+                              as_h8(codes<1>(x0), codes<1>(y0), codes<1>(x1), codes<1>(y1))};
+            uint32_t pw[4];   // keys i and i + 2 of each half
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int u = k / 2, i = k % 2;
+                const float p0 = sc[u][i], p1 = sc[u][i + 2];
+                const float d0 = half_of(cv.d[u][b][0], i), d1 = half_of(cv.d[u][b][1], i);
+                uint32_t hi = word_of((_Float16) __builtin_fmaf(p0, d0, 0.0f), (_Float16) __builtin_fmaf(p1, d1, 0.0f));
+                if (NS == 2) {
+                    // (one rounding of the product for both uses: the compiler may round it in one step or in two)
+                    asm volatile("" : "+v"(hi));
+                    const uint32_t lo = word_of((_Float16) __builtin_fmaf(p0, d0, -half_of(hi, 0)),
+                                                (_Float16) __builtin_fmaf(p1, d1, -half_of(hi, 1)));
+                    hi = m < RC ? hi : lo;
+                }
+                pw[k] = hi;
+            }
+            if (masked)   // (a masked key's scale may be a NaN)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int key = key0 + 16 * (k / 2) + k % 2;
+                    pw[k] &= (key <= see ? 0xffffu : 0u) | (key + 2 <= see ? 0xffff0000u : 0u);
+                }
+            const h8 pb = as_h8(pw[0], pw[1], pw[2], pw[3]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) o[2 * b + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[k], pb, o[2 * b + k], 0, 0, 0);
+        }
+        if (BUF == 1 && next < c1) nv.load(cell, l);
+        c = next;
+    };
+    while (c < c1) {
+        turn(0);
+        if (BUF == 1) continue;
+        if (c >= c1) break;
+        turn(1);
+    }
+
+    // the waves' sums meet in LDS
+    lsum += __shfl_xor(lsum, 16);
+    lsum += __shfl_xor(lsum, 32);
+    if (l < RC) {
+        s_off[w][l] = off;
+        s_l[w][l] = lsum;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) {
+        if (NS == 2)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] += other_part(o[i][j]);
+        if (m < RC) *(f4*) (s_o + (w * RC + m) * LD + 16 * i + 4 * g) = o[i];
+    }
+    __syncthreads();
+    const int ways = 1 << cshift, tiles = 1 << tshift;
+    for (int e = tid; e < rows * (D / 4); e += 64 * W) {
+        const int row = e / (D / 4), dim = 4 * (e % (D / 4)), tile = row / RC, rr = row % RC;
+        float at = NO_KEY, sum = 0.0f;
+        for (int k = 0; k < ways; ++k) at = fmaxf(at, s_off[tile + tiles * k][rr]);
+        f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < ways; ++k) {
+            const int from = tile + tiles * k;
+            const float f = exp2_hw(s_off[from][rr] - at);
+            v += *(const f4*) (s_o + (from * RC + rr) * LD + dim) * f;
+            sum += s_l[from][rr] * f;
+        }
+        v *= 512.0f;
+        const int tok = (int) ((unsigned) row / R), hh = hd * (int) R + (int) ((unsigned) row % R), lastc = (back + tok) >> 5;
+        if (lastc < a.cells) {          // the row's keys are all in the first split
+            if (z > 0) continue;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            q4_put4((char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1, a.type, hh * D + dim, v * inv);
+        } else if (zc <= lastc) {
+            const int64_t p = (((int64_t) z * a.S + s.i) * a.tcap + tok) * a.n_head + hh;
+            *(f4*) (a.part + p * D + dim) = v;
+            if (dim == 0) *(float2*) (a.stat + 2 * p) = float2{at, sum};
+        }
+    }
+}
+
+// ---- many rows per request ------------------------------------------------------
+//
+// A workgroup of eight waves takes 16-column tiles of a request's rows and one kv head.  Here
+// a cell serves many tiles, so its values are formed once, d (code - 8) itself, as matrix
+// core operands in LDS: no scaling around the products then, and a weight enters once, not
+// once per block.  The product of an 11-bit scale and a 4-bit code has 15 bits: f32 and f16
+// rows take it exactly as two f16 parts (EXACT), bf16 rows as one, whose 2^-12 is far below
+// their own rounding.  Scales are brought into f16's range by powers of two, 2^sk and 2^sv,
+// that only fall, where some cell's largest scale asks for it (every wave looks at every
+// scale, so all agree without exchange).
+//
+// D <= 128: four waves' rows, two tiles each, and two cells at a time, one per half of the waves,
+// whose sums meet in LDS at the end; D = 256: eight waves' rows, a tile each, one cell at a time.
+// Two buffers: the next step's operands are formed, and the one after's dwords loaded, while this
+// one's are used; one barrier a step.
+//
+// A NaN scale of a value is taken as 0 and its block set to NaN afterwards in the rows that
+// see the key: 0 times NaN would reach those that do not.
+constexpr int qr_tiles(int D) { return D == 256 ? 1 : 2; }
+constexpr int qr_halves(int D) { return D == 256 ? 1 : 2; }
+
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+    h2 x, y;
+    __builtin_memcpy(&x, &a, 4);
+    __builtin_memcpy(&y, &b, 4);
+    x = x * y;
+    __builtin_memcpy(&a, &x, 4);
+    return a;
+}
+// a b - c, rounded once
+__device__ __forceinline__ uint32_t rest_h2(uint32_t a, uint32_t b, uint32_t c) {
+    h2 x, y, v;
+    __builtin_memcpy(&x, &a, 4);
+    __builtin_memcpy(&y, &b, 4);
+    __builtin_memcpy(&v, &c, 4);
+    x = __builtin_elementwise_fma(x, y, -v);
+    __builtin_memcpy(&a, &x, 4);
+    return a;
+}
+__device__ __forceinline__ uint32_t pow2_h2(int e) {   // 2^e in both halves, -14 <= e <= 15
+    const uint32_t x = (uint32_t) (e + 15) << 10;
+    return x | x << 16;
+}
+
+template <int D, int NS, bool EXACT>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) k_attn_q4_rows(AttnQ4Args a, int most) {
+    constexpr int NB = D / 32, RC = 16 / NS, NC = qr_tiles(D), KH = qr_halves(D), RG = 8 / KH, RW = NC * RC, RB = RG * RW;
+    constexpr int RN = 8 / KH, PF = 2 * NB / RN;                // waves that form a cell's operands, K (and V) operands of each
+    constexpr int PARTS = EXACT ? 2 : 1, FR = 4 * NB;           // a cell: FR operands of 64 lanes x 16 bytes per part
+    __shared__ __align__(16) uint8_t s_mem[2 * KH * PARTS * FR * 1024];
+    __shared__ float s_off[4][NC][64], s_l[4][NC][64];
+    const int tid = threadIdx.x, l = tid & 63, m = l & 15, g = l >> 4;
+    const int w = uni(tid >> 6), rg = w % RG, kh = w / RG, role = w % RN;
+    const unsigned R = (unsigned) a.n_head / (unsigned) a.c.n_head_kv;
+    const int hd = blockIdx.y, z = blockIdx.z;
+    Q4Seq s;
+    if (!q4_find(a, l, blockIdx.x, [&](int t, int i) { return (int64_t) max(t, 0) * R / RB + i; }, s)) return;
+    const int rows = (int) min((int64_t) s.n * R, (int64_t) 1 << 30);
+    if (rows <= most) return;                                   // (k_attn_q4's)
+    // the request's blocks, the last rows (the most keys) first
+    const int blocks = (rows + RB - 1) / RB, at = blockIdx.x - (int) ((int64_t) s.row0 * R / RB + s.i);
+    if (at >= blocks) return;
+    const int base = (blocks - 1 - at) * RB;
+    int len = s.len;
+    if (!q4_fits(a, s)) {
+        len = 0;
+        if (tid == 0) atomicOr(a.status, QWMOE_STATUS_BAD_SEQ);
+    }
+    const int r0 = base + rg * RW, wrows = max(min(rows - r0, RW), 0), back = len - s.n;
+    const int block_last = back + (int) ((unsigned) (min(rows, base + RB) - 1) / R);
+    const int last = wrows ? back + (int) ((unsigned) (r0 + wrows - 1) / R) : -1;
+    const int every = back + (int) ((unsigned) r0 / R);
+    const int zc = (int) min((int64_t) z * a.row_cells, (int64_t) 1 << 30);
+    if (z > 0 && zc > block_last >> 5) return;
+    const int cend = block_last < 0 ? zc : (int) min(zc + a.row_cells, (int64_t) (block_last >> 5) + 1);   // cells zc .. cend - 1
+    const int steps = (cend - zc + KH - 1) / KH;
+
+    const int32_t* pages = a.table + (int64_t) s.i * a.W;
+    const int cpp = a.c.page_shift - 5;
+    const uint8_t* head = a.c.data + hd * a.c.head_bytes();
+    const int64_t page_bytes = a.c.page_bytes();
+    // pages of 64 cells at a time, one per lane
+    int pg = 0, pg_at = zc;
+    auto fetch_pages = [&](int c) {
+        pg_at = c;
+        pg = c + l < cend ? pages[(c + l) >> cpp] : 0;
+        if (pg < 0 || pg >= a.c.n_pages) {
+            atomicOr(a.status, QWMOE_STATUS_BAD_SLOT);
+            pg = -1;
+        }
+    };
+    // this wave's share of a step: one cell's dwords, and all of the step's scales
+    uint32_t kc[PF], vc[2], vd[2][2], chk[KH][2][(NB + 3) / 4];
+    uint16_t kd[PF];
+    int page[KH];
+    const int kf = role * PF, ku = kf / NB, kb = kf % NB;       // its K operands: half ku, blocks kb ..
+    const int vb = role * PF / 2;                               // its V operands: block vb (with one operand: half role % 2)
+    auto load = [&](int step) __attribute__((always_inline)) {
+        const int c = zc + step * KH;
+        if (c + KH - 1 - pg_at >= 64) fetch_pages(c);
+#pragma unroll
+        for (int k = 0; k < KH; ++k) {
+            const int ck = min(c + k, cend - 1);
+            page[k] = c + k < cend ? __builtin_amdgcn_readlane(pg, ck - pg_at) : -1;
+            const uint8_t* cell = head + max(page[k], 0) * page_bytes + (ck & ((1 << cpp) - 1)) * (36 * D);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if constexpr (NB == 2) chk[k][e][0] = *(const uint16_t*) (cell + (uint32_t) ((e ? 34 : 16) * D + 2 * l));
+                else __builtin_memcpy(chk[k][e], cell + (uint32_t) ((e ? 34 : 16) * D + NB * l), NB);
+            if (w / RN == k) {
+                __builtin_memcpy(kc, cell + (uint32_t) ((((16 * ku + m) * 4 + g) * NB + kb) * 4), 4 * PF);
+#pragma unroll
+                for (int j = 0; j < PF; ++j)
+                    kd[j] = *(const uint16_t*) (cell + (uint32_t) (16 * D + (((4 * ku + (m >> 2)) * NB + kb + j) * 4 + (m & 3)) * 2));
+                __builtin_memcpy(vc, cell + (uint32_t) (18 * D + ((((vb >> 1) * 16 + m) * 4 + g) * 2 + (vb & 1)) * 8), 8);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) __builtin_memcpy(vd[u], cell + (uint32_t) (34 * D + ((4 * u + g) * NB + vb) * 8), 8);
+            }
+        }
+    };
+    int sk = 15, sv = 15;                                       // of the operands formed last
+    int nans = 0, gone = 0;                                     // bit k: cell k of it holds a NaN value scale; has no page
+    auto operand = [&](int buf, int cellk, int part, int f) {
+        return s_mem + ((((buf * KH + cellk) * PARTS + part) * FR + f) * 64 + l) * 16;
+    };
+    auto form = [&](int step, int buf) __attribute__((always_inline)) {
+        const int c = zc + step * KH;
+        // the powers of two: 2^15 or less of the largest scale below 2^14
+        nans = gone = 0;
+        uint32_t top[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < KH; ++k) {
+            if (page[k] < 0) gone |= 1 << k;
+            const int keys = page[k] < 0 ? 0 : len - 32 * (c + k);
+            uint32_t any_nan = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < NB / 2; ++j) {
+                    uint32_t x = (chk[k][e][j / 2] >> (16 * (j & 1))) & 0x7fffu;
+                    const int idx = l * (NB / 2) + j, key = 4 * (idx / (4 * NB)) + idx % 4;
+                    x = key < keys ? x : 0u;
+                    if (e) any_nan |= x > 0x7c00u;
+                    top[e] = max(top[e], x > 0x7c00u ? 0u : x);
+                }
+            if (__any(any_nan)) nans |= 1 << k;
+        }
+        auto settle = [&](uint32_t t, int& sh) {
+            // |d| 2^sh < 2^15, that is exponent(d) + sh <= 14
+            if (!__any((int) (t >> 10) - 15 + sh > 14)) return;
+#pragma unroll
+            for (int k = 32; k >= 1; k >>= 1) t = max(t, (uint32_t) __shfl_xor((int) t, k));
+            sh = uni(14 + 15 - (int) (t >> 10));
+        };
+        settle(top[0], sk);
+        settle(top[1], sv);
+        const int mine = w / RN, keys = gone >> mine & 1 ? 0 : len - 32 * (c + mine);   // its cell, the request's keys in it
+#pragma unroll
+        for (int j = 0; j < PF; ++j) {
+            const uint32_t d = mul_h2((uint32_t) kd[j] * 0x10001u, pow2_h2(sk)), c4 = kc[j], d4 = c4 >> 8;
+            const uint32_t cc[4] = {codes<0>(c4), codes<1>(c4), codes<0>(d4), codes<1>(d4)};
+            uint32_t hi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[e] = mul_h2(cc[e], d);
+            *(u32x4*) operand(buf, mine, 0, kf + j) = u32x4{hi[0], hi[1], hi[2], hi[3]};
+            if constexpr (EXACT)
+                *(u32x4*) operand(buf, mine, 1, kf + j) =
+                    u32x4{rest_h2(cc[0], d, hi[0]), rest_h2(cc[1], d, hi[1]), rest_h2(cc[2], d, hi[2]), rest_h2(cc[3], d, hi[3])};
+        }
+        uint32_t d[4];   // of keys (0, 2), (1, 3) of both halves
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            uint32_t x0 = vd[u][0], x1 = vd[u][1];
+            if (keys < 32 || (nans >> mine & 1)) {   // keys behind the request's, NaNs: 0
+                const int k0 = 16 * u + 4 * g;
+                auto keep = [&](uint32_t x, int key) {
+                    const uint32_t lo = (x & 0x7fffu) <= 0x7c00u && key < keys ? x & 0xffffu : 0u;
+                    const uint32_t hi = (x >> 16 & 0x7fffu) <= 0x7c00u && key + 1 < keys ? x & 0xffff0000u : 0u;
+                    return lo | hi;
+                };
+                x0 = keep(x0, k0);
+                x1 = keep(x1, k0 + 2);
+            }
+            d[2 * u] = mul_h2(__builtin_amdgcn_perm(x1, x0, 0x05040100u), pow2_h2(sv));
+            d[2 * u + 1] = mul_h2(__builtin_amdgcn_perm(x1, x0, 0x07060302u), pow2_h2(sv));
+        }
+        const uint32_t x0 = vc[0], x1 = vc[1], y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (PF == 1 && half != (role & 1)) continue;
+            const uint32_t cc[4] = {half ? codes<1>(x0) : codes<0>(x0), half ? codes<1>(y0) : codes<0>(y0),
+                                    half ? codes<1>(x1) : codes<0>(x1), half ? codes<1>(y1) : codes<0>(y1)};
+            uint32_t hi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[e] = mul_h2(cc[e], d[e]);
+            const int f = 2 * NB + 2 * vb + half;
+            *(u32x4*) operand(buf, mine, 0, f) = u32x4{hi[0], hi[1], hi[2], hi[3]};
+            if constexpr (EXACT)
+                *(u32x4*) operand(buf, mine, 1, f) = u32x4{rest_h2(cc[0], d[0], hi[0]), rest_h2(cc[1], d[1], hi[1]),
+                                                           rest_h2(cc[2], d[2], hi[2]), rest_h2(cc[3], d[3], hi[3])};
+        }
+    };
+    if (steps > 0) {
+        fetch_pages(zc);
+        load(0);
+    }
+
+    // this lane's rows
+    int lim[NC];
+    h8 q[NC][NB];
+    float qs[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const int r = r0 + n * RC + (m & (RC - 1));
+        const bool ok = r < rows;
+        const int t = ok ? (int) ((unsigned) r / R) : 0, h = ok ? hd * (int) R + (int) ((unsigned) r % R) : 0;
+        lim[n] = ok ? back + t : -1;
+        qs[n] = 512.0f * q4_load_q<D, NS>(a, s.row0 + t, h, ok, l, q[n]);
+    }
+    f4 o[NC][2 * NB];            // O^T 2^(osv - 9)
+    float off[NC], mx[NC], lsum[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        off[n] = mx[n] = NO_KEY;
+        lsum[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) o[n][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int osv = 15;
+    if (steps > 0) form(0, 0);
+    if (steps > 1) load(1);
+    for (int step = 0; step < steps; ++step) {
+        const int buf = step & 1, c = zc + step * KH + kh;
+        const int csk = sk, csv = sv;
+        const bool nan_here = nans >> kh & 1, work = !(gone >> kh & 1) && 32 * c <= last;   // some row of the wave sees the cell
+        lds_barrier();   // this step's operands are there; the other buffer's readers are done
+        if (step + 1 < steps) {
+            form(step + 1, buf ^ 1);
+            if (step + 2 < steps) load(step + 2);
+        }
+        if (!work) continue;
+        const bool masked = 32 * c + 31 > every;                // some row does not see some key of the cell
+        const int key0 = 32 * c + 4 * g;                        // key i of half u: key0 + 16 u + i
+        f4 sc[NC][2];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) sc[n][0] = sc[n][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const h8 ka = *(const h8*) operand(buf, kh, p, u * NB + b);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[n][b], sc[n][u], 0, 0, 0);
+                }
+        const float unit = bitsf((uint32_t) (127 - csk) << 23);
+        if (csv != osv) {
+            const float f = bitsf((uint32_t) (127 + csv - osv) << 23);
+            osv = csv;
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int i = 0; i < 2 * NB; ++i) o[n][i] *= f;
+        }
+        u32x4 pw[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const float qn = qs[n] * unit;
+            if (NS == 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sc[n][i / 4][i % 4] += other_part(sc[n][i / 4][i % 4]);
+            if (masked)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sc[n][i / 4][i % 4] = key0 + 16 * (i / 4) + i % 4 <= lim[n] ? sc[n][i / 4][i % 4] : -INFINITY;
+            float smax = sc[n][0][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) smax = fmaxf(smax, sc[n][i / 4][i % 4]);
+            if (__any(__builtin_fmaf(smax, qn, -off[n]) > 12.0f)) {
                 smax = fmaxf(smax, __shfl_xor(smax, 16));
                 smax = fmaxf(smax, __shfl_xor(smax, 32));
-                mx[n] = fmaxf(mx[n], smax * qs[n]);
-                const float now = mx[n] == NO_KEY ? NO_KEY : mx[n] + (float) (E - 4);
-                const float f = exp2_hw(off[n] - now);
+                mx[n] = fmaxf(mx[n], smax * qn);
+                const float now = mx[n] == NO_KEY ? NO_KEY : mx[n] - 4.0f, f = exp2_hw(off[n] - now);
                 off[n] = now;
                 lsum[n] *= f;
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) o[n][i] *= f;
             }
-        }
-        // weights, formed in place
+            float p[8];
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            if (n && n >= wtiles) continue;
+            for (int i = 0; i < 8; ++i) {
+                p[i] = exp2_hw(__builtin_fmaf(sc[n][i / 4][i % 4], qn, -off[n]));
+                lsum[n] += p[i];
+            }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = exp2_hw(__builtin_fmaf(sc[n][u][i], qs[n], -off[n]));
-                    sc[n][u][i] = p;
-                    lsum[n] += p;
+            for (int k = 0; k < 4; ++k) {   // keys i and i + 2 of each half
+                const float p0 = p[4 * (k / 2) + k % 2], p1 = p[4 * (k / 2) + k % 2 + 2];
+                uint32_t hi = word_of((_Float16) p0, (_Float16) p1);
+                if (NS == 2) {
+                    const uint32_t lo = word_of((_Float16) (p0 - half_of(hi, 0)), (_Float16) (p1 - half_of(hi, 1)));
+                    hi = m < RC ? hi : lo;
                 }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            h8 va[2];
-            {
-                const uint32_t x0 = x.v[b][0], x1 = x.v[b][1], y0 = x0 >> 8, y1 = x1 >> 8;
-                va[0] = as_h8(codes<0>(x0), codes<0>(y0), codes<0>(x1), codes<0>(y1));
-                va[1] = as_h8(codes<1>(x0), codes<1>(y0), codes<1>(x1), codes<1>(y1));
-            }
-#pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                if (n && n >= wtiles) continue;
-                uint32_t pw[4];
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {   // keys i and i + 2
-                        const float p0 = sc[n][u][i], p1 = sc[n][u][i + 2];
-                        float d0 = half_of(x.vs[u][b][0], i), d1 = half_of(x.vs[u][b][1], i);
-                        if (MASK) {   // (a masked key's scale may be a NaN)
-                            const int key = 32 * c + 16 * u + 4 * g + i;
-                            d0 = !gone && key <= lim[n] ? d0 : 0.0f;
-                            d1 = !gone && key + 2 <= lim[n] ? d1 : 0.0f;
-                        }
-                        uint32_t hi = word_of((_Float16) (p0 * d0), (_Float16) (p1 * d1));
-                        if (NS == 2) {
-                            // (one rounding of the product for both uses: the compiler may round it in one step or in two)
-                            asm volatile("" : "+v"(hi));
-                            const uint32_t lo = word_of((_Float16) __builtin_fmaf(p0, d0, -half_of(hi, 0)),
-                                                        (_Float16) __builtin_fmaf(p1, d1, -half_of(hi, 1)));
-                            hi = m < RC ? hi : lo;
-                        }
-                        pw[2 * u + i] = hi;
-                    }
-                const h8 pb = as_h8(pw[0], pw[1], pw[2], pw[3]);
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    o[n][2 * b + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[k], pb, o[n][2 * b + k], 0, 0, 0);
+                pw[n][k] = hi;
             }
         }
-    };
-    {
-        Q4Cell<D> x[2];
-        int page[2] = {0, 0};
-        int c = c0;
-        if (c < c1) {
-            fetch_pages(c);
-            page[0] = page_of(c);
-            x[0].load(address(c, page[0]), l);
-        }
-        auto turn = [&](int now) __attribute__((always_inline)) {
-            const int next = c + (1 << cshift);
-            if (next < c1) {
-                if ((next - pg_at) >> cshift >= 64) fetch_pages(next);
-                page[now ^ 1] = page_of(next);
-                x[now ^ 1].load(address(next, page[now ^ 1]), l);
+#pragma unroll
+        for (int f = 0; f < 2 * NB; ++f)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const h8 va = *(const h8*) operand(buf, kh, p, 2 * NB + f);
+#pragma unroll
+                for (int n = 0; n < NC; ++n)
+                    o[n][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, as_h8(pw[n][0], pw[n][1], pw[n][2], pw[n][3]), o[n][f], 0, 0, 0);
             }
-            const bool gone = page[now] < 0;
-            if (32 * c + 31 <= every && !gone) step(x[now], c, false, std::false_type{});
-            else step(x[now], c, gone, std::true_type{});
-            c = next;
-        };
-        while (c < c1) {
-            turn(0);
-            if (c >= c1) break;
-            turn(1);
+        if (nan_here) {
+            const uint8_t* cell = head + (int64_t) pages[c >> cpp] * page_bytes + (c & ((1 << cpp) - 1)) * (36 * D);
+            for (int t = 0; t < 32; ++t)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const uint16_t d = *(const uint16_t*) (cell + 34 * D + (((t >> 2) * NB + b) * 4 + (t & 3)) * 2);
+                    if ((d & 0x7fffu) <= 0x7c00u) continue;
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+                        if (32 * c + t <= lim[n])
+                            o[n][2 * b] = o[n][2 * b + 1] = f4{NAN, NAN, NAN, NAN};
+                }
         }
     }
 
-    // a row's results: out, or the split's sums
-    const int64_t heads = a.T * a.n_head;
-    auto put = [&](int64_t row, int lm, int dim, f4 v, float sum, float at) {
-        const int parts = lm < 0 ? 1 : (int) ((lm >> 5) / a.cells) + 1;
-        if (z >= parts) return;
-        if (parts == 1) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            char* dst = (char*) a.out + (row / a.n_head) * (int64_t) a.out_nb1;
-            q4_put4(dst, a.type, (row % a.n_head) * D + dim, v * inv);
-        } else {
-            const int64_t p = z * heads + row;
-            *(f4*) (a.part + p * D + dim) = v;
-            if (dim == 0) *(float2*) (a.stat + 2 * p) = float2{at, sum};
-        }
-    };
+    const float unit = bitsf((uint32_t) (127 + 9 - osv) << 23);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         lsum[n] += __shfl_xor(lsum[n], 16);
         lsum[n] += __shfl_xor(lsum[n], 32);
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
-            o[n][i] *= 512.0f;
+            o[n][i] *= unit;
             if (NS == 2)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[n][i][j] += other_part(o[n][i][j]);
         }
     }
-    if (!share) {
+    if constexpr (KH == 2) {   // the second half's sums to the first
+        lds_barrier();
+        if (kh == 1) {
 #pragma unroll
-        for (int n = 0; n < NC; ++n)
-            if (orow[n] >= 0 && m < RC)
+            for (int n = 0; n < NC; ++n) {
+                s_off[rg][n][l] = off[n];
+                s_l[rg][n][l] = lsum[n];
 #pragma unroll
-                for (int i = 0; i < 2 * NB; ++i) put(orow[n], lim[n], 16 * i + 4 * g, o[n][i], lsum[n], off[n]);
-        return;
+                for (int i = 0; i < 2 * NB; ++i) *(f4*) (s_mem + (((rg * NC + n) * 2 * NB + i) * 64 + l) * 16) = o[n][i];
+            }
+        }
+        lds_barrier();
+        if (kh == 1) return;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const float other = s_off[rg][n][l], now = fmaxf(off[n], other), f0 = exp2_hw(off[n] - now), f1 = exp2_hw(other - now);
+            off[n] = now;
+            lsum[n] = lsum[n] * f0 + s_l[rg][n][l] * f1;
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i)
+                o[n][i] = o[n][i] * f0 + *(const f4*) (s_mem + (((rg * NC + n) * 2 * NB + i) * 64 + l) * 16) * f1;
+        }
     }
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
-        if (g == 0 && m < RC) {
-            s_off[w][n * RC + m] = off[n];
-            s_l[w][n * RC + m] = lsum[n];
-        }
-#pragma unroll
     for (int n = 0; n < NC; ++n) {
-        if (n * RC >= wrows) break;   // uniform over the workgroup
-        __syncthreads();
-        if (m < RC)
+        const int r = r0 + n * RC + m;
+        if (m >= RC || r >= rows) continue;
+        const int tok = (int) ((unsigned) r / R), h = hd * (int) R + (int) ((unsigned) r % R), lastc = (back + tok) >> 5;
+        if (lastc < a.row_cells) {   // the row's keys are all in the first split
+            if (z > 0) continue;
+            const float inv = lsum[n] == 0.0f ? 0.0f : 1.0f / lsum[n];
+            char* dst = (char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1;
 #pragma unroll
-            for (int i = 0; i < 2 * NB; ++i) *(f4*) (s_o + (w * RC + m) * LD + 16 * i + 4 * g) = o[n][i];
-        __syncthreads();
-        for (int e = tid; e < RC * (D / 4); e += 256) {
-            const int rr = e / (D / 4), dim = 4 * (e % (D / 4)), r = n * RC + rr;
-            if (r >= wrows) break;
-            const float at = fmaxf(fmaxf(s_off[0][r], s_off[1][r]), fmaxf(s_off[2][r], s_off[3][r]));
-            f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            float sum = 0.0f;
+            for (int i = 0; i < 2 * NB; ++i) q4_put4(dst, a.type, h * D + 16 * i + 4 * g, o[n][i] * inv);
+        } else if (zc <= lastc) {
+            const int64_t p = ((int64_t) z * a.T + s.row0 + tok) * a.n_head + h;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float f = exp2_hw(s_off[k][r] - at);
-                v += *(const f4*) (s_o + (k * RC + rr) * LD + dim) * f;
-                sum += s_l[k][r] * f;
-            }
-            const int64_t rq = r0 + r;
-            const int t = (int) (rq / R);
-            put((s.row0 + t) * a.n_head + hd * R + (int) (rq % R), back + t, dim, v, sum, at);
+            for (int i = 0; i < 2 * NB; ++i) *(f4*) (a.row_part + p * D + 16 * i + 4 * g) = o[n][i];
+            if (g == 0) *(float2*) (a.row_stat + 2 * p) = float2{off[n], lsum[n]};
         }
     }
 }
@@ -514,18 +848,12 @@ __global__ void __launch_bounds__(256) k_attn_q4(AttnQ4Args a) {
 // A row's splits, joined: a workgroup per row, D / 4 lanes per split; each lane adds every
 // WAYS-th split in order, then the ways are added in order.
 template <int D>
-__global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
+__device__ __forceinline__ void q4_join(const AttnQ4Args& a, int tok, int h, int parts, const float* part, const float* stat, int64_t row,
+                                        int64_t heads) {
     constexpr int LN = D / 4, WAYS = 256 / LN;
     __shared__ __align__(16) f4 s_v[256];
     __shared__ float s_at[WAYS], s_sum[WAYS];
     const int tid = threadIdx.x, way = tid / LN, dim = 4 * (tid % LN);
-    const int64_t heads = a.T * a.n_head, row = blockIdx.x, tok = row / a.n_head;
-    Q4Seq s;
-    if (!q4_request(a, q4_last(a.S, tid & 63, [&](int i) { return a.seq_start[i] <= tok; }), s)) return;
-    if (tok >= s.row0 + s.n || !q4_fits(a, s)) return;
-    const int lim = s.len - s.n + (int) (tok - s.row0);
-    const int parts = lim < 0 ? 1 : (int) ((lim >> 5) / a.cells) + 1;
-    if (parts == 1) return;
     f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
     float at = NO_KEY, sum = 0.0f;
     auto add = [&](const f4& pv, float pat, float psum) __attribute__((always_inline)) {
@@ -537,8 +865,8 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
 #pragma unroll 4
     for (int z = way; z < parts; z += WAYS) {
         const int64_t p = z * heads + row;
-        const float2 st = *(const float2*) (a.stat + 2 * p);
-        add(*(const f4*) (a.part + p * D + dim), st.x, st.y);
+        const float2 st = *(const float2*) (stat + 2 * p);
+        add(*(const f4*) (part + p * D + dim), st.x, st.y);
     }
     s_v[tid] = v;
     if (dim == 0) {
@@ -549,49 +877,83 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a) {
     if (way > 0) return;
     for (int k = 1; k < WAYS; ++k) add(s_v[k * LN + tid], s_at[k], s_sum[k]);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    q4_put4((char*) a.out + tok * (int64_t) a.out_nb1, a.type, (row % a.n_head) * D + dim, v * inv);
+    q4_put4((char*) a.out + (int64_t) tok * a.out_nb1, a.type, h * D + dim, v * inv);
+}
+__device__ __forceinline__ int q4_parts(int lim, int64_t cells) { return lim < 0 ? 1 : (int) ((unsigned) (lim >> 5) / (unsigned) cells) + 1; }
+
+// of k_attn_q4: workgroups (request, head, token)
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a, int most) {
+    Q4Seq s;
+    const int h = blockIdx.y, t = blockIdx.z;
+    if (!q4_request(a, blockIdx.x, s) || t >= s.n || !q4_fits(a, s) || (int64_t) s.n * (a.n_head / a.c.n_head_kv) > most) return;
+    const int parts = q4_parts(s.len - s.n + t, a.cells);
+    if (parts > 1)
+        q4_join<D>(a, s.row0 + t, h, parts, a.part, a.stat, ((int64_t) s.i * a.tcap + t) * a.n_head + h, (int64_t) a.S * a.tcap * a.n_head);
+}
+// of k_attn_q4_rows: workgroups (token row, head)
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int most) {
+    Q4Seq s;
+    const int h = blockIdx.y, tok = blockIdx.x;
+    if (!q4_find(a, threadIdx.x & 63, tok, [](int t, int) { return (int64_t) t; }, s)) return;
+    if (tok >= s.row0 + s.n || !q4_fits(a, s) || (int64_t) s.n * (a.n_head / a.c.n_head_kv) <= most) return;
+    const int parts = q4_parts(s.len - s.n + (tok - s.row0), a.row_cells);
+    if (parts > 1)
+        q4_join<D>(a, tok, h, parts, a.row_part, a.row_stat, (int64_t) tok * a.n_head + h, a.T * a.n_head);
 }
 
-template <int D, int NS, int NC>
+template <int D, int NS>
 int launch(const AttnQ4Args& a, hipStream_t st) {
-    const int64_t blocks = q4_blocks(a, 4 * NC * (16 / NS));
-    if (blocks > 0x7fffffff) return -2;
-    const dim3 g((unsigned) blocks, (unsigned) a.c.n_head_kv, (unsigned) a.splits);
-    hipLaunchKernelGGL((k_attn_q4<D, NS, NC>), g, dim3(256), 0, st, a);
-    if (a.splits > 1) hipLaunchKernelGGL(k_attn_q4_join<D>, dim3((unsigned) (a.T * a.n_head)), dim3(256), 0, st, a);
+    constexpr int W = q4_group(D), few = W * (16 / NS);
+    const int64_t R = a.n_head / a.c.n_head_kv;
+    const unsigned nk = (unsigned) a.c.n_head_kv;
+    hipLaunchKernelGGL((k_attn_q4<D, NS>), dim3((unsigned) a.S, nk, (unsigned) a.splits), dim3(64 * W), 0, st, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL(k_attn_q4_join<D>, dim3((unsigned) a.S, (unsigned) a.n_head, (unsigned) a.tcap), dim3(256), 0, st, a, few);
+    if (std::min(a.max_new, a.T) * R > few) {
+        const int64_t blocks = q4_row_blocks(a);
+        if (blocks > 0x7fffffff) return -2;
+        const dim3 g((unsigned) blocks, nk, (unsigned) a.row_splits);
+        if (a.type == KV_BF16) {
+            if constexpr (NS == 1) hipLaunchKernelGGL((k_attn_q4_rows<D, 1, false>), g, dim3(512), 0, st, a, few);
+        } else hipLaunchKernelGGL((k_attn_q4_rows<D, NS, true>), g, dim3(512), 0, st, a, few);
+        if (a.row_splits > 1)
+            hipLaunchKernelGGL(k_attn_q4_rows_join<D>, dim3((unsigned) a.T, (unsigned) a.n_head), dim3(256), 0, st, a, few);
+    }
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
-template <int D, int NS>
-int launch_tiles(const AttnQ4Args& a, hipStream_t st) {
-    switch (q4_tiles(a)) {
-        case 1: return launch<D, NS, 1>(a, st);
-        case 2: return launch<D, NS, 2>(a, st);
-        default:
-            if constexpr (D < 256) return launch<D, NS, 4>(a, st);
-            else return -2;
-    }
-}
+
+int parts_of(const AttnQ4Args& a) { return a.type == KV_F32 ? 8 : 16; }   // rows of a 16-column tile
+int few_of(const AttnQ4Args& a) { return q4_group(a.c.D) * parts_of(a); }
 
 }  // namespace
 
-int q4_tiles(const AttnQ4Args& a) {
-    const int64_t rows = std::min<int64_t>(a.max_new, a.T) * (a.n_head / a.c.n_head_kv), per = a.type == KV_F32 ? 8 : 16;
-    return rows <= per ? 1 : rows <= 2 * per || a.c.D == 256 ? 2 : 4;
+int64_t q4_few_tokens(const AttnQ4Args& a) {
+    return std::min<int64_t>(std::min(a.max_new, a.T), few_of(a) / (a.n_head / a.c.n_head_kv));
 }
-int64_t q4_blocks(const AttnQ4Args& a, int per) { return a.T * (a.n_head / a.c.n_head_kv) / per + a.S; }
 int64_t q4_splits(const AttnQ4Args& a) {
-    const int64_t per = (int64_t) 4 * q4_tiles(a) * (a.type == KV_F32 ? 8 : 16);
-    const int64_t groups = q4_blocks(a, (int) per) * a.c.n_head_kv, cells = (a.max_len + KV_CELL - 1) / KV_CELL;
-    return std::max<int64_t>(1, std::min<int64_t>({512 / groups, cells / 8, 4096}));
+    if (q4_few_tokens(a) == 0) return 1;
+    const int64_t groups = (int64_t) a.S * a.c.n_head_kv, cells = (a.max_len + KV_CELL - 1) / KV_CELL;
+    return std::max<int64_t>(1, std::min<int64_t>({512 / groups, cells / 16, 4096}));
+}
+int64_t q4_row_blocks(const AttnQ4Args& a) {
+    const int per = 8 / qr_halves(a.c.D) * qr_tiles(a.c.D) * parts_of(a);
+    return a.T * (a.n_head / a.c.n_head_kv) / per + a.S;
+}
+int64_t q4_row_splits(const AttnQ4Args& a) {
+    if (std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) <= few_of(a)) return 1;
+    const int64_t groups = q4_row_blocks(a) * a.c.n_head_kv, cells = (a.max_len + KV_CELL - 1) / KV_CELL;
+    return std::max<int64_t>(1, std::min<int64_t>(256 / groups, cells / 16));
 }
 
 int launch_attn_q4(const AttnQ4Args& a, hipStream_t st) {
     if (a.T == 0) return 0;
     const bool two = a.type == KV_F32;
     switch (a.c.D) {
-        case 64: return two ? launch_tiles<64, 2>(a, st) : launch_tiles<64, 1>(a, st);
-        case 128: return two ? launch_tiles<128, 2>(a, st) : launch_tiles<128, 1>(a, st);
-        default: return two ? launch_tiles<256, 2>(a, st) : launch_tiles<256, 1>(a, st);
+        case 64: return two ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
+        case 128: return two ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
+        default: return two ? launch<256, 2>(a, st) : launch<256, 1>(a, st);
     }
 }
 

@@ -81,15 +81,21 @@ struct AttnQ4Args {
     const int32_t *table, *seq_start, *seq_len;
     int64_t max_new, max_len;
     float scale;                          // of the scores, times log2(e)
-    int64_t cells;                        // cells of 32 keys per split
+    // requests of few rows: cells of 32 keys per split, and where there is more than one, their
+    // sums [splits][S][tcap][n_head][D] and [..][2] offset and sum of weights
+    int64_t cells, tcap;
     int splits;
-    float *part, *stat;                   // [splits][T][n_head][D] sums and [..][2] offset, sum of weights (splits > 1)
+    float *part, *stat;
+    // the others: likewise, [row_splits][T][n_head][..]
+    int64_t row_cells;
+    int row_splits;
+    float *row_part, *row_stat;
     int32_t* status;
 };
-// Tiles of 16 columns per wave, blocks of `per` rows, and how many splits of the keys fill the card.
-int q4_tiles(const AttnQ4Args& a);
-int64_t q4_blocks(const AttnQ4Args& a, int per);
-int64_t q4_splits(const AttnQ4Args& a);
+int64_t q4_few_tokens(const AttnQ4Args& a);   // new tokens, at most, of a request of few rows
+int64_t q4_splits(const AttnQ4Args& a);       // splits of the keys that fill the card
+int64_t q4_row_splits(const AttnQ4Args& a);
+int64_t q4_row_blocks(const AttnQ4Args& a);
 int launch_attn_q4(const AttnQ4Args& a, hipStream_t stream);
 
 }  // namespace qw

@@ -11,6 +11,7 @@ half a step of their type; attention to a bound derived from its roundings:
   weights   2 delta, exp2 and the sums over len keys: (len + 64) 2^-24 + 2^-21; f16 and bf16
             rows round each weight to f16: 2^-11; weights far below the largest are
             f16 subnormals: 2^-28 of it each;
+  bf16      requests of many rows: keys and values rounded once to f16, 2^-11 each (B 2^-11 in delta);
   values    all of it times sum p |v| (and len max |v| for the last), the codes being exact;
   output    half a step of its type.
 """
@@ -303,8 +304,9 @@ class Batch:
             a = int(self.start[i])
             g = got[a:a + n].double().cpu().numpy()
             want, mag, big = orc.attention(self.q64[a:a + n], self.k64[i], self.v64[i], n, scale)
-            delta = big * ((self.D + 16) * 2.0**-24 + 2.0**-21)
-            tol = mag * (2 * delta * (1 + delta) + (length + 64) * 2.0**-24 + 2.0**-21 + (0 if self.typ == torch.float32 else 2.0**-11))
+            bf16 = 2.0**-11 if self.typ == torch.bfloat16 else 0.0
+            delta = big * ((self.D + 16) * 2.0**-24 + 2.0**-21 + bf16)
+            tol = mag * (2 * delta * (1 + delta) + (length + 64) * 2.0**-24 + 2.0**-21 + (0 if self.typ == torch.float32 else 2.0**-11) + bf16)
             vmax = np.abs(self.v64[i]).max() if length else 0.0
             tol = tol + length * vmax * 2.0**-28 + np.abs(want) * (torch.finfo(self.typ).eps / 2) + 2.0**-25
             for r, heads in but:
