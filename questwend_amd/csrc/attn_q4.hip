@@ -47,7 +47,7 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float NO_KEY = -3.0e38f;   // M and off of a row that has seen no key yet
 
@@ -586,35 +586,50 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
     auto form = [&](int step, int buf) __attribute__((always_inline)) {
         const int c = zc + step * KH;
-        // the powers of two: 2^15 or less of the largest scale below 2^14
+        // the powers of two: every scale below 2^15 after them.  One comparison per kind says that they stand (keys
+        // behind the request's may fail it for nothing)
         nans = gone = 0;
-        uint32_t top[2] = {0, 0};
+        u16x2 raw[2] = {u16x2{0, 0}, u16x2{0, 0}};
 #pragma unroll
         for (int k = 0; k < KH; ++k) {
             if (page[k] < 0) gone |= 1 << k;
-            const int keys = page[k] < 0 ? 0 : len - 32 * (c + k);
-            uint32_t any_nan = 0;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int j = 0; j < NB / 2; ++j) {
-                    uint32_t x = (chk[k][e][j / 2] >> (16 * (j & 1))) & 0x7fffu;
-                    const int idx = l * (NB / 2) + j, key = 4 * (idx / (4 * NB)) + idx % 4;
-                    x = key < keys ? x : 0u;
-                    if (e) any_nan |= x > 0x7c00u;
-                    top[e] = max(top[e], x > 0x7c00u ? 0u : x);
+                for (int j = 0; j < (NB + 3) / 4; ++j) {
+                    const uint32_t x = chk[k][e][j] & 0x7fff7fffu;
+                    u16x2 y;
+                    __builtin_memcpy(&y, &x, 4);
+                    raw[e] = __builtin_elementwise_max(raw[e], y);
                 }
-            if (__any(any_nan)) nans |= 1 << k;
         }
-        auto settle = [&](uint32_t t, int& sh) {
-            // |d| 2^sh < 2^15, that is exponent(d) + sh <= 14
-            if (!__any((int) (t >> 10) - 15 + sh > 14)) return;
+        const bool fails = max((int) raw[0][0], (int) raw[0][1]) >= (30 - sk) << 10 || max((int) raw[1][0], (int) raw[1][1]) >= (30 - sv) << 10;
+        if (__any(fails)) {
+            uint32_t top[2] = {0, 0};
 #pragma unroll
-            for (int k = 32; k >= 1; k >>= 1) t = max(t, (uint32_t) __shfl_xor((int) t, k));
-            sh = uni(14 + 15 - (int) (t >> 10));
-        };
-        settle(top[0], sk);
-        settle(top[1], sv);
+            for (int k = 0; k < KH; ++k) {
+                const int keys = page[k] < 0 ? 0 : len - 32 * (c + k);
+                bool any_nan = false;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < NB / 2; ++j) {
+                        uint32_t x = (chk[k][e][j / 2] >> (16 * (j & 1))) & 0x7fffu;
+                        const int idx = l * (NB / 2) + j, key = 4 * (idx / (4 * NB)) + idx % 4;
+                        x = key < keys ? x : 0u;
+                        if (e) any_nan |= x > 0x7c00u;
+                        top[e] = max(top[e], x > 0x7c00u ? 0u : x);
+                    }
+                if (__any(any_nan)) nans |= 1 << k;
+            }
+            auto settle = [&](uint32_t t, int& sh) {
+#pragma unroll
+                for (int k = 32; k >= 1; k >>= 1) t = max(t, (uint32_t) __shfl_xor((int) t, k));
+                sh = min(sh, uni(29 - (int) (t >> 10)));   // exponent(d) + sh <= 14
+            };
+            settle(top[0], sk);
+            settle(top[1], sv);
+        }
         const int mine = w / RN, keys = gone >> mine & 1 ? 0 : len - 32 * (c + mine);   // its cell, the request's keys in it
 #pragma unroll
         for (int j = 0; j < PF; ++j) {
@@ -688,29 +703,25 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int i = 0; i < 2 * NB; ++i) o[n][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     int osv = 15;
-    if (steps > 0) form(0, 0);
-    if (steps > 1) load(1);
-    for (int step = 0; step < steps; ++step) {
-        const int buf = step & 1, c = zc + step * KH + kh;
-        const int csk = sk, csv = sv;
-        const bool nan_here = nans >> kh & 1, work = !(gone >> kh & 1) && 32 * c <= last;   // some row of the wave sees the cell
-        lds_barrier();   // this step's operands are there; the other buffer's readers are done
+    auto ahead = [&](int step) __attribute__((always_inline)) {
         if (step + 1 < steps) {
-            form(step + 1, buf ^ 1);
+            form(step + 1, (step & 1) ^ 1);
             if (step + 2 < steps) load(step + 2);
         }
-        if (!work) continue;
+    };
+    auto multiply = [&](int buf, int c, int csk, int csv, bool nan_here) __attribute__((always_inline)) {
         const bool masked = 32 * c + 31 > every;                // some row does not see some key of the cell
         const int key0 = 32 * c + 4 * g;                        // key i of half u: key0 + 16 u + i
         f4 sc[NC][2];
 #pragma unroll
         for (int n = 0; n < NC; ++n) sc[n][0] = sc[n][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        // (products that add to one register stand four apart)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
+                for (int u = 0; u < 2; ++u) {
                     const h8 ka = *(const h8*) operand(buf, kh, p, u * NB + b);
 #pragma unroll
                     for (int n = 0; n < NC; ++n) sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[n][b], sc[n][u], 0, 0, 0);
@@ -766,14 +777,16 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
             }
         }
 #pragma unroll
-        for (int f = 0; f < 2 * NB; ++f)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                const h8 va = *(const h8*) operand(buf, kh, p, 2 * NB + f);
+            for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                for (int n = 0; n < NC; ++n)
-                    o[n][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, as_h8(pw[n][0], pw[n][1], pw[n][2], pw[n][3]), o[n][f], 0, 0, 0);
-            }
+                for (int f = 2 * b; f < 2 * b + 2; ++f) {
+                    const h8 va = *(const h8*) operand(buf, kh, p, 2 * NB + f);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+                        o[n][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, as_h8(pw[n][0], pw[n][1], pw[n][2], pw[n][3]), o[n][f], 0, 0, 0);
+                }
         if (nan_here) {
             const uint8_t* cell = head + (int64_t) pages[c >> cpp] * page_bytes + (c & ((1 << cpp) - 1)) * (36 * D);
             for (int t = 0; t < 32; ++t)
@@ -787,8 +800,19 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
                             o[n][2 * b] = o[n][2 * b + 1] = f4{NAN, NAN, NAN, NAN};
                 }
         }
+    };
+    if (steps > 0) form(0, 0);
+    if (steps > 1) load(1);
+    for (int step = 0; step < steps; ++step) {
+        const int buf = step & 1, c = zc + step * KH + kh;
+        const int csk = sk, csv = sv;
+        const bool nan_here = nans >> kh & 1, work = !(gone >> kh & 1) && 32 * c <= last;   // some row of the wave sees the cell
+        lds_barrier();   // this step's operands are there; the other buffer's readers are done
+        // one of a SIMD's two waves forms operands while the other multiplies
+        if (w < 4) ahead(step);
+        if (work) multiply(buf, c, csk, csv, nan_here);
+        if (w >= 4) ahead(step);
     }
-
     const float unit = bitsf((uint32_t) (127 + 9 - osv) << 23);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -903,15 +927,18 @@ __global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int mos
         q4_join<D>(a, tok, h, parts, a.row_part, a.row_stat, (int64_t) tok * a.n_head + h, a.T * a.n_head);
 }
 
+// Requests of up to `few` rows are k_attn_q4's, the others k_attn_q4_rows' (a lone request that may have more rows: too).
 template <int D, int NS>
 int launch(const AttnQ4Args& a, hipStream_t st) {
-    constexpr int W = q4_group(D), few = W * (16 / NS);
-    const int64_t R = a.n_head / a.c.n_head_kv;
+    constexpr int W = q4_group(D);
+    const int few = a.tcap > 0 ? W * (16 / NS) : 0;
     const unsigned nk = (unsigned) a.c.n_head_kv;
-    hipLaunchKernelGGL((k_attn_q4<D, NS>), dim3((unsigned) a.S, nk, (unsigned) a.splits), dim3(64 * W), 0, st, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL(k_attn_q4_join<D>, dim3((unsigned) a.S, (unsigned) a.n_head, (unsigned) a.tcap), dim3(256), 0, st, a, few);
-    if (std::min(a.max_new, a.T) * R > few) {
+    if (few) {
+        hipLaunchKernelGGL((k_attn_q4<D, NS>), dim3((unsigned) a.S, nk, (unsigned) a.splits), dim3(64 * W), 0, st, a);
+        if (a.splits > 1)
+            hipLaunchKernelGGL(k_attn_q4_join<D>, dim3((unsigned) a.S, (unsigned) a.n_head, (unsigned) a.tcap), dim3(256), 0, st, a, few);
+    }
+    if (std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) > few) {
         const int64_t blocks = q4_row_blocks(a);
         if (blocks > 0x7fffffff) return -2;
         const dim3 g((unsigned) blocks, nk, (unsigned) a.row_splits);
@@ -923,13 +950,13 @@ int launch(const AttnQ4Args& a, hipStream_t st) {
     }
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
-
 int parts_of(const AttnQ4Args& a) { return a.type == KV_F32 ? 8 : 16; }   // rows of a 16-column tile
 int few_of(const AttnQ4Args& a) { return q4_group(a.c.D) * parts_of(a); }
 
 }  // namespace
 
 int64_t q4_few_tokens(const AttnQ4Args& a) {
+    if (a.S == 1 && std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) > few_of(a)) return 0;
     return std::min<int64_t>(std::min(a.max_new, a.T), few_of(a) / (a.n_head / a.c.n_head_kv));
 }
 int64_t q4_splits(const AttnQ4Args& a) {
