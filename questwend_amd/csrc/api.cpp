@@ -1119,6 +1119,8 @@ int qwmoe_attn_kv_q4(void* stream, const qwmoe_kv_q4* cache, int type, const voi
     a.q_nb1 = q_nb1;
     a.out_nb1 = out_nb1;
     a.n_head = (int) n_head;
+    a.group = (int) (n_head / cache->n_head_kv);
+    a.group_inv = (uint32_t) (((uint64_t) 1 << 32) / (uint64_t) a.group + 1);   // (not used for 1)
     a.S = (int) n_seq;
     a.T = n_tokens;
     a.W = table_width;

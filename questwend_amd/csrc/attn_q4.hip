@@ -37,6 +37,7 @@
 
 #include "../../include/qwmoe.h"
 #include "qw_kv_q4.hpp"
+#include "qw_mfma.hpp"
 
 namespace qw {
 
@@ -46,6 +47,7 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
@@ -55,6 +57,12 @@ __device__ __forceinline__ void q4_put4(void* p, int type, int64_t i, f4 v) {
     if (type == KV_F32) *(f4*) ((float*) p + i) = v;
     else if (type == KV_F16) *(h4*) ((_Float16*) p + i) = __builtin_convertvector(v, h4);
     else *(b4*) ((__bf16*) p + i) = __builtin_convertvector(v, b4);
+}
+
+__device__ __forceinline__ void q4_put2(void* p, int type, int i, float x, float y) {
+    if (type == KV_F32) *(float2*) ((float*) p + i) = float2{x, y};
+    else if (type == KV_F16) *(h2*) ((_Float16*) p + i) = h2{(_Float16) x, (_Float16) y};
+    else *(b2*) ((__bf16*) p + i) = b2{(__bf16) x, (__bf16) y};
 }
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -101,48 +109,19 @@ __device__ __forceinline__ bool q4_fits(const AttnQ4Args& a, const Q4Seq& s) {
     return s.len >= 0 && s.len <= a.max_len && s.n <= a.max_new;
 }
 
-// One cell's dwords as they lie in memory: keys, values.
+// A cell's copy into LDS: instructions of 64 x 16 bytes, the rest of 64 x 4.
 template <int D>
-struct Q4Keys {
-    static constexpr int NB = D / 32;
-    uint32_t c[2][NB];       // codes of token l % 16 of both halves, dims 8 (l / 16) .. of each block
-    uint32_t d[2][NB][2];    // scales of keys 4 (l / 16) .. + 3 of both halves
-    __device__ __forceinline__ void load(const uint8_t* cell, int l) {
-        const int m = l & 15, g = l >> 4;
+struct Q4Copy {
+    static constexpr int BYTES = 36 * D, WIDE = BYTES / 1024, INSTR = WIDE + BYTES % 1024 / 256;
+    static __device__ __forceinline__ void issue(const uint8_t* cell, uint8_t* slot, int l) {
+        const i32x4 r = rsrc_words(cell, BYTES);
+        const i32x4 rs = i32x4{uni(r.x), uni(r.y), uni(r.z), uni(r.w)};
+        uint32_t lb = (uint32_t) uni((int) (uint32_t) (uintptr_t) slot);
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(lb)::"memory");   // (the slot's last reads are done)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            __builtin_memcpy(c[u], cell + (uint32_t) (((16 * u + m) * 4 + g) * NB * 4), 4 * NB);
-            __builtin_memcpy(d[u], cell + (uint32_t) (16 * D + (4 * u + g) * NB * 8), 8 * NB);
-        }
-    }
-};
-template <int D>
-struct Q4Values {
-    static constexpr int NB = D / 32;
-    uint32_t c[NB][2];           // codes of dims l % 16 and 16 + l % 16 of each block, keys 4 (l / 16) .. of both halves
-    uint32_t d[2][NB][2];        // scales of the same keys
-    uint32_t chk[(NB + 3) / 4];  // the lane's share of the scales (NB / 2 halves)
-    __device__ __forceinline__ void load(const uint8_t* cell, int l) {
-        const int m = l & 15, g = l >> 4;
+        for (int j = 0; j < WIDE; ++j) dma_b128(rs, lb + 1024u * j, (uint32_t) (16 * l + 1024 * j), 0u);
 #pragma unroll
-        for (int b = 0; b < NB; b += 2)
-            __builtin_memcpy(c[b], cell + (uint32_t) (18 * D + (((b / 2) * 16 + m) * 4 + g) * 16), 16);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) __builtin_memcpy(d[u], cell + (uint32_t) (34 * D + (4 * u + g) * NB * 8), 8 * NB);
-        if constexpr (NB == 2) chk[0] = *(const uint16_t*) (cell + (uint32_t) (34 * D + 2 * l));
-        else __builtin_memcpy(chk, cell + (uint32_t) (34 * D + NB * l), NB);
-    }
-    // the largest magnitude among the lane's share, of keys below `keys`, as f16 bits; NaNs count as 0
-    __device__ __forceinline__ uint32_t top(int l, int keys) const {
-        uint32_t t = 0;
-#pragma unroll
-        for (int e = 0; e < NB / 2; ++e) {
-            uint32_t x = (chk[e / 2] >> (16 * (e & 1))) & 0x7fffu;
-            const int at = l * (NB / 2) + e, key = 4 * (at / (4 * NB)) + at % 4;
-            x = x > 0x7c00u || key >= keys ? 0u : x;
-            t = max(t, x);
-        }
-        return t;
+        for (int j = 0; j < INSTR - WIDE; ++j) dma_b32(rs, lb + 1024u * WIDE + 256u * j, (uint32_t) (4 * l + 1024 * WIDE + 256 * j), 0u);
     }
 };
 
@@ -175,79 +154,117 @@ __device__ __forceinline__ uint32_t codes(uint32_t w) {
     return w;
 }
 
+// The values of lanes l ^ 16 and l ^ 32 join this lane's: all four groups of 16 then agree.
+template <typename F>
+__device__ __forceinline__ float over_groups(float v, F join) {
+    auto a = __builtin_amdgcn_permlane16_swap(fbits(v), fbits(v), false, false);
+    v = join(bitsf(a[0]), bitsf(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(fbits(v), fbits(v), false, false);
+    return join(bitsf(b[0]), bitsf(b[1]));
+}
+__device__ __forceinline__ float max_over_16(float v) {
+    v = fmaxf(v, dpp_f<0x121>(v));   // row_ror 1, 2, 4, 8
+    v = fmaxf(v, dpp_f<0x122>(v));
+    v = fmaxf(v, dpp_f<0x124>(v));
+    return fmaxf(v, dpp_f<0x128>(v));
+}
+__device__ __forceinline__ float max_over_groups(float v) {
+    return over_groups(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_over_groups(float v) {
+    return over_groups(v, [](float a, float b) { return a + b; });
+}
+// The largest of all lanes' values below 2^16.
+__device__ __forceinline__ int max_of_wave(int v) {
+    v = max(v, dpp_i<0x121>(v));   // row_ror 1, 2, 4, 8
+    v = max(v, dpp_i<0x122>(v));
+    v = max(v, dpp_i<0x124>(v));
+    v = max(v, dpp_i<0x128>(v));
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
 // (lane l ^ 8 of the same 16)
 __device__ __forceinline__ float other_part(float v) { return dpp_f<0x128>(v); }   // row_ror:8
 
-// Waves of a workgroup, and per SIMD, that the registers leave room for; two cells' dwords in flight
-// where they fit.
-constexpr int q4_group(int D) { return D == 256 ? 4 : 8; }
-constexpr int q4_simd(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }
-constexpr int q4_buffers(int D) { return D <= 128 ? 2 : 1; }
+// Waves of a workgroup: as many as the registers hold, a workgroup to a CU.  Cells of a wave in flight or in
+// use: as many as LDS holds.
+constexpr int q4_waves(int D) { return 8; }
+constexpr int q4_ring(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
+constexpr int Q4_TILES = 8;   // of a request that k_attn_q4 takes
 
 // A row's q (NS f16 parts; lane l has dims 8 (l / 16) .. of each block, f32 rows' low parts in
-// columns 8 .. 15), scaled by a power of two into f16's upper range; returns the scores'
-// factor: scale log2(e) over that power.
+// columns 8 .. 15): its dwords, then the parts, scaled by a power of two into f16's upper range.
+// parts() returns the scores' factor: scale log2(e) over that power.
 template <int D, int NS>
-__device__ __forceinline__ float q4_load_q(const AttnQ4Args& a, int tok, int h, bool ok, int l, h8 (&q)[D / 32]) {
-    constexpr int NB = D / 32;
-    float x[NB][8];
-    const char* src = (const char*) a.q + (int64_t) tok * a.q_nb1;
-    const int at = h * D + 8 * (l >> 4);
-    if constexpr (NS == 2) {
+struct Q4Row {
+    static constexpr int NB = D / 32;
+    u32x4 x[NB][NS];
+    __device__ __forceinline__ void load(const AttnQ4Args& a, int tok, int h, int l) {
+        const char* src = (const char*) a.q + (int64_t) tok * a.q_nb1 + (uint32_t) (h * D + 8 * (l >> 4)) * (2 * NS);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const f4 lo = *(const f4*) ((const float*) src + at + 32 * b), hi = *(const f4*) ((const float*) src + at + 32 * b + 4);
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[b][j] = j < 4 ? lo[j & 3] : hi[j & 3];
-        }
-    } else {
-        const bool f16 = a.type == KV_F16;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const u32x4 v = *(const u32x4*) ((const uint16_t*) src + at + 32 * b);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t word = v[j / 2];
-                x[b][j] = f16 ? half_of(word, j & 1) : bitsf(j & 1 ? word & 0xffff0000u : word << 16);
-            }
-        }
+            for (int e = 0; e < NS; ++e) x[b][e] = *(const u32x4*) (src + 64 * NS * b + 16 * e);
     }
-    float big = 0.0f;
+    __device__ __forceinline__ float parts(const AttnQ4Args& a, bool ok, int l, h8 (&q)[NB]) const {
+        const bool f16 = a.type == KV_F16;
+        auto value = [&](int b, int j) {
+            if constexpr (NS == 2) return bitsf(x[b][j / 4][j % 4]);
+            const uint32_t word = x[b][0][j / 2];
+            return f16 ? half_of(word, j & 1) : bitsf(j & 1 ? word & 0xffff0000u : word << 16);
+        };
+        float big = 0.0f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) big = fmaxf(big, __builtin_fabsf(x[b][j]));
-    big = fmaxf(big, __shfl_xor(big, 16));
-    big = fmaxf(big, __shfl_xor(big, 32));
-    // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
-    const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
-    const float up = ok ? bitsf((uint32_t) (127 + 14 - ex) << 23) : 0.0f;
+            for (int j = 0; j < 8; ++j) big = fmaxf(big, __builtin_fabsf(value(b, j)));
+        big = max_over_groups(big);
+        // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
+        const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
+        const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+            uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float y = x[b][j] * up;
-            const _Float16 v = (_Float16) y;
-            q[b][j] = NS == 2 && (l & 15) >= 8 ? (_Float16) (y - (float) v) : v;
+            for (int j = 0; j < 4; ++j) {
+                const float y0 = value(b, 2 * j) * up, y1 = value(b, 2 * j + 1) * up;
+                w[j] = word_of((_Float16) y0, (_Float16) y1);
+                if (NS == 2) {
+                    const uint32_t lo = word_of((_Float16) (y0 - half_of(w[j], 0)), (_Float16) (y1 - half_of(w[j], 1)));
+                    w[j] = (l & 8) ? lo : w[j];
+                }
+                w[j] = ok ? w[j] : 0u;
+            }
+            q[b] = as_h8(w[0], w[1], w[2], w[3]);
         }
-    return a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
-}
+        return a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
+    }
+};
 
 // NS f16 parts per row (f32 rows: two).
 template <int D, int NS>
-__global__ void __launch_bounds__(64 * q4_group(D)) __attribute__((amdgpu_waves_per_eu(q4_simd(D), q4_simd(D)))) k_attn_q4(AttnQ4Args a) {
-    constexpr int NB = D / 32, RC = 16 / NS, W = q4_group(D), BUF = q4_buffers(D);
-    constexpr int LD = D + 4;                                   // floats of a row in LDS
-    __shared__ __align__(16) float s_o[W * RC * LD];
-    __shared__ float s_off[W][RC], s_l[W][RC];
+__global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_per_eu(q4_waves(D) / 4, q4_waves(D) / 4))) k_attn_q4(AttnQ4Args a) {
+    constexpr int NB = D / 32, RC = 16 / NS, W = q4_waves(D), N = q4_ring(D), I = Q4Copy<D>::INSTR, SLOT = Q4Copy<D>::BYTES;
+    constexpr int LD = D + 4;                                   // floats of a row where the waves' sums meet
+    __shared__ __align__(16) uint8_t s_ring[W * (N * SLOT > RC * LD * 4 ? N * SLOT : RC * LD * 4)];
+    __shared__ float2 s_ol[W][RC];                              // offset and sum of weights
+    constexpr int LQ = D + 8;                                   // halves of a row's q
+    __shared__ float s_qs[RC * Q4_TILES];
     const int tid = threadIdx.x, l = tid & 63, m = l & 15, g = l >> 4;
     const int w = uni(tid >> 6);
-    const unsigned R = (unsigned) a.n_head / (unsigned) a.c.n_head_kv;
-    const int hd = blockIdx.y, z = blockIdx.z;
+    const int R = a.group, hd = blockIdx.y, z = blockIdx.z;
+    auto by_R = [&](int r) { return R == 1 ? r : (int) __umulhi((unsigned) r, a.group_inv); };   // r / R for 0 <= r < 2^16
+    // pages of the split's cells, 64 at a time, one per lane (entries behind the request's are read, not used: they
+    // come in with its lengths)
+    const int32_t* pages = a.table + (int64_t) blockIdx.x * a.W;
+    const int cpp = a.c.page_shift - 5;                         // log2 of a page's cells
+    const int zc = (int) min((int64_t) z * a.cells, (int64_t) 1 << 30);
+    int pg_at = zc >> cpp, pg = pages[min((int64_t) pg_at + l, a.W - 1)];
     Q4Seq s;
     if (!q4_request(a, blockIdx.x, s)) return;
     const int rows = (int) min((int64_t) s.n * R, (int64_t) 1 << 30);
-    if (rows > W * RC) return;                                  // (k_attn_q4_rows')
+    if (rows > Q4_TILES * RC) return;                           // (k_attn_q4_rows')
     int len = s.len;
     if (!q4_fits(a, s)) {
         len = 0;
@@ -255,78 +272,113 @@ __global__ void __launch_bounds__(64 * q4_group(D)) __attribute__((amdgpu_waves_
     }
     // the waves of the workgroup: 2^tshift tiles of rows, 2^cshift waves each
     const int tshift = rows <= RC ? 0 : rows <= 2 * RC ? 1 : rows <= 4 * RC ? 2 : 3;
-    const int cshift = (W == 8 ? 3 : 2) - tshift;
+    const int cshift = (W == 16 ? 4 : 3) - tshift;
     const int r0 = (w & ((1 << tshift) - 1)) * RC;              // the wave's first row
     const int wrows = max(min(rows - r0, RC), 0);
     const int back = len - s.n;                                 // a row of token t sees keys .. back + t
-    const int last = wrows ? back + (int) ((unsigned) (r0 + wrows - 1) / R) : -1;   // the last key some row of the wave sees
-    const int every = back + (int) ((unsigned) r0 / R);         // keys up to here are seen by all of its rows
+    const int last = wrows ? back + by_R(r0 + wrows - 1) : -1;  // the last key some row of the wave sees
+    const int every = back + by_R(r0);                          // keys up to here are seen by all of its rows
     const int cells = last < 0 ? 0 : (last >> 5) + 1;
-    const int zc = (int) min((int64_t) z * a.cells, (int64_t) 1 << 30);
     if (z > 0 && zc > (len - 1) >> 5) return;                   // (z = 0 writes the rows without keys)
     const int c0 = min(zc + (w >> tshift), cells);              // its cells: c0, c0 + 2^cshift ..
     const int c1 = (int) min(zc + a.cells, (int64_t) cells);
 
-    // cells: their pages, 64 of the wave's at a time, one per lane
-    const int32_t* pages = a.table + (int64_t) s.i * a.W;
-    const int cpp = a.c.page_shift - 5;                         // log2 of a page's cells
-    int pg = 0, pg_at = c0;
-    auto fetch_pages = [&](int c) {
-        pg_at = c;
-        const int mine = c + (l << cshift);
-        pg = mine < c1 ? pages[mine >> cpp] : 0;
-        if (pg < 0 || pg >= a.c.n_pages) {
-            atomicOr(a.status, QWMOE_STATUS_BAD_SLOT);
-            pg = -1;
-        }
-    };
-    auto page_of = [&](int c) { return __builtin_amdgcn_readlane(pg, (c - pg_at) >> cshift); };
-    const uint8_t* head = a.c.data + hd * a.c.head_bytes();
-    const int64_t page_bytes = a.c.page_bytes();
-    auto address = [&](int c, int page) { return head + max(page, 0) * page_bytes + (c & ((1 << cpp) - 1)) * (36 * D); };
-    Q4Keys<D> xk[BUF];
-    Q4Values<D> xv[BUF];
-    int c = c0, page = 0;
-    if (c < c1) {
-        fetch_pages(c);
-        page = page_of(c);
-        const uint8_t* cell = address(c, page);
-        xk[0].load(cell, l);
-        xv[0].load(cell, l);
-    }
-
     // this lane's row
     const int r = r0 + (m & (RC - 1));
     const bool ok = r < rows;
-    const int t = ok ? (int) ((unsigned) r / R) : 0, h = ok ? hd * (int) R + (int) ((unsigned) r % R) : 0;
-    const int lim = ok ? back + t : -1;                         // the last key it sees
+    const int lim = ok ? back + by_R(r) : -1;                   // the last key it sees
+    const uint8_t* head = a.c.data + hd * a.c.head_bytes();
+    const int64_t page_bytes = a.c.page_bytes();
+    uint8_t* ring = s_ring + w * SLOT;                          // [slot][wave]
+    uint32_t bad = 0;                                           // bit k: the cell in slot k has no page
+    auto issue = [&](int c, int slot) __attribute__((always_inline)) {
+        if ((c >> cpp) - pg_at >= 64) {
+            pg_at = c >> cpp;
+            pg = pages[min((int64_t) pg_at + l, a.W - 1)];
+        }
+        const int page = __builtin_amdgcn_readlane(pg, (c >> cpp) - pg_at);
+        const bool ok = page >= 0 && page < a.c.n_pages;
+        if (!ok && l == 0) atomicOr(a.status, QWMOE_STATUS_BAD_SLOT);
+        bad = ok ? bad & ~(1u << slot) : bad | 1u << slot;
+        Q4Copy<D>::issue(head + (ok ? page : 0) * page_bytes + (c & ((1 << cpp) - 1)) * (36 * D), ring + slot * (W * SLOT), l);
+    };
+#pragma unroll
+    for (int k = 0; k < N - 1; ++k)
+        if (c0 + (k << cshift) < c1) issue(c0 + (k << cshift), k);
+
+    // q, a row per wave in turn: scaled by a power of two into f16's upper range, its parts to LDS (where the
+    // rings' last slots, still unused, are)
+    _Float16* s_q = (_Float16*) (s_ring + (N - 1) * W * SLOT);
+    static_assert(NS * RC * Q4_TILES * LQ * 2 <= W * SLOT, "q fits the last slots");
+    for (int i = w; i < (RC << tshift); i += W) {
+        const bool there = i < rows;
+        const int t = there ? by_R(i) : 0, h = there ? hd * R + i - t * R : 0;
+        constexpr int E = D / 64;                               // values of a lane
+        float x[E], big = 0.0f;
+        const char* src = (const char*) a.q + (int64_t) (s.row0 + t) * a.q_nb1 + (h * D + E * l) * (2 * NS);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if constexpr (NS == 2) x[e] = ((const float*) src)[e];
+            else x[e] = a.type == KV_F16 ? (float) ((const _Float16*) src)[e] : bitsf((uint32_t) ((const uint16_t*) src)[e] << 16);
+            big = fmaxf(big, __builtin_fabsf(x[e]));
+        }
+        big = max_over_groups(max_over_16(big));
+        // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
+        const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
+        const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
+        _Float16* dst = s_q + i * LQ + E * l;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float y = there ? x[e] * up : 0.0f;
+            const _Float16 hi = (_Float16) y;
+            dst[e] = hi;
+            if (NS == 2) dst[8 * Q4_TILES * LQ + e] = (_Float16) (y - (float) hi);
+        }
+        if (l == 0) s_qs[i] = 512.0f * a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
+    }
+    lds_barrier();   // (the cells' copies stay in flight)
     h8 q[NB];
-    const float qs = 512.0f * q4_load_q<D, NS>(a, s.row0 + t, h, ok, l, q);
+    {
+        const _Float16* src = s_q + ((NS == 2 && m >= RC ? 8 * Q4_TILES : 0) + r0 + (m & (RC - 1))) * LQ + 8 * g;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) q[b] = *(const h8*) (src + 32 * b);
+    }
+    lds_barrier();
+    const float qs = s_qs[r0 + (m & (RC - 1))];                 // the scores' factor: scale log2(e), 2^9 for the codes, q's power of two
 
     f4 o[2 * NB];                // O^T 2^-9: dims 16 tile + 4 g + i of the lane's row
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     float off = NO_KEY, mx = NO_KEY, lsum = 0.0f;
     int E = -25;                 // the value scales so far are at most 2^E
-    uint32_t Ebits = 0;          // 2^E as f16 bits
+    int Ebits = 0;               // 2^E as f16 bits
 
-    // one cell; with two buffers the next one's loads go out first, with one buffer its keys' when these
-    // are used and its values' likewise
-    auto turn = [&](int now) __attribute__((always_inline)) {
-        Q4Keys<D>&ck = xk[now % BUF], &nk = xk[(now + 1) % BUF];
-        Q4Values<D>&cv = xv[now % BUF], &nv = xv[(now + 1) % BUF];
-        const int next = c + (1 << cshift);
-        const uint8_t* cell = nullptr;
-        const bool gone = page < 0;
-        if (next < c1) {
-            if ((next - pg_at) >> cshift >= 64) fetch_pages(next);
-            page = page_of(next);
-            cell = address(next, page);
-            if (BUF == 2) {
-                nk.load(cell, l);
-                nv.load(cell, l);
-            }
+    const uint32_t high = m < RC ? 0xffffffffu : 0u;            // lanes with high parts
+    int slot = 0;
+    for (int c = c0; c < c1; c += 1 << cshift) {
+        const int ahead = c + ((N - 1) << cshift);
+        const bool gone = bad >> slot & 1;
+        if (ahead < c1) {
+            issue(ahead, slot == 0 ? N - 1 : slot - 1);
+            vm_wait<(N - 1) * I>();
+        } else if (N > 2 && c + ((N - 2) << cshift) < c1) vm_wait<(N > 2 ? N - 2 : 0) * I>();
+        else if (N > 3 && c + ((N - 3) << cshift) < c1) vm_wait<(N > 3 ? N - 3 : 0) * I>();
+        else vm_wait<0>();
+        const uint8_t* cell = ring + slot * (W * SLOT);
+        slot = slot == N - 1 ? 0 : slot + 1;
+        uint32_t kc[2][NB], kd[2][NB][2], vc[NB][2], vd[2][NB][2], chk[(NB + 3) / 4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            __builtin_memcpy(kc[u], __builtin_assume_aligned(cell + ((16 * u + m) * 4 + g) * NB * 4, NB == 2 ? 8 : 16), 4 * NB);
+            __builtin_memcpy(kd[u], __builtin_assume_aligned(cell + 16 * D + (4 * u + g) * NB * 8, 16), 8 * NB);
         }
+        if constexpr (NB == 2) chk[0] = *(const uint16_t*) (cell + 34 * D + 2 * l);
+        else __builtin_memcpy(chk, __builtin_assume_aligned(cell + 34 * D + NB * l, NB), NB);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) __builtin_memcpy(vd[u], __builtin_assume_aligned(cell + 34 * D + (4 * u + g) * NB * 8, 16), 8 * NB);
+#pragma unroll
+        for (int b = 0; b < NB; b += 2)
+            __builtin_memcpy(vc[b], __builtin_assume_aligned(cell + 18 * D + (((b / 2) * 16 + m) * 4 + g) * 16, 16), 16);
         const bool masked = 32 * c + 31 > every || gone;        // some row does not see some key of the cell
         const int key0 = 32 * c + 4 * g, see = gone ? -1 : lim; // key i of half u: key0 + 16 u + i
         f4 sc[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
@@ -334,13 +386,20 @@ __global__ void __launch_bounds__(64 * q4_group(D)) __attribute__((amdgpu_waves_
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const uint32_t c4 = ck.c[u][b], d4 = c4 >> 8;
+                const uint32_t c4 = kc[u][b], d4 = c4 >> 8;
                 const h8 ka = as_h8(codes<0>(c4), codes<1>(c4), codes<0>(d4), codes<1>(d4));
                 const f4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[b], f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[u][i] = __builtin_fmaf(p[i], half_of(ck.d[u][b][i / 2], i & 1), sc[u][i]);
+                for (int i = 0; i < 4; ++i) sc[u][i] = __builtin_fmaf(p[i], half_of(kd[u][b][i / 2], i & 1), sc[u][i]);
             }
-        if (BUF == 1 && next < c1) nk.load(cell, l);
+        // the largest value scale of the request's keys, as f16 bits (NaNs count as 0), from the lane's share
+        int top = 0;
+#pragma unroll
+        for (int e = 0; e < NB / 2; ++e) {
+            const int x = (int) (chk[e / 2] >> (16 * (e & 1))) & 0x7fff;
+            const int at = l * (NB / 2) + e, key = 4 * (at / (4 * NB)) + at % 4;
+            top = max(top, x > 0x7c00 || key > last - 32 * c ? 0 : x);
+        }
         if (NS == 2)
 #pragma unroll
             for (int i = 0; i < 8; ++i) sc[i / 4][i % 4] += other_part(sc[i / 4][i % 4]);
@@ -350,22 +409,15 @@ __global__ void __launch_bounds__(64 * q4_group(D)) __attribute__((amdgpu_waves_
         float smax = sc[0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) smax = fmaxf(smax, sc[i / 4][i % 4]);
-        const uint32_t top = cv.top(l, last + 1 - 32 * c);
         if (__any(top > Ebits || __builtin_fmaf(smax, qs, -off) > 12.0f - (float) E)) {
-            uint32_t t = top;
-#pragma unroll
-            for (int k = 32; k >= 1; k >>= 1) t = max(t, (uint32_t) __shfl_xor((int) t, k));
-            t = (uint32_t) uni((int) t);
+            const int t = max_of_wave(top);
             if (t > Ebits) {   // the power of two above the largest scale (from 2^-14 on, f16's smallest normal number)
-                E = max((int) (t >> 10), 1) - 14;
-                Ebits = (uint32_t) (E + 15) << 10;
+                E = max(t >> 10, 1) - 14;
+                Ebits = (E + 15) << 10;
             }
-            smax = fmaxf(smax, __shfl_xor(smax, 16));
-            smax = fmaxf(smax, __shfl_xor(smax, 32));
-            mx = fmaxf(mx, smax * qs);
-            const float now_off = mx == NO_KEY ? NO_KEY : mx + (float) (E - 4);
-            const float f = exp2_hw(off - now_off);
-            off = now_off;
+            mx = fmaxf(mx, max_over_groups(smax) * qs);
+            const float now = mx == NO_KEY ? NO_KEY : mx + (float) (E - 4), f = exp2_hw(off - now);
+            off = now;
             lsum *= f;
 #pragma unroll
             for (int i = 0; i < 2 * NB; ++i) o[i] *= f;
@@ -379,81 +431,84 @@ __global__ void __launch_bounds__(64 * q4_group(D)) __attribute__((amdgpu_waves_
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const uint32_t x0 = cv.c[b][0], x1 = cv.c[b][1], y0 = x0 >> 8, y1 = x1 >> 8;
+            const uint32_t x0 = vc[b][0], x1 = vc[b][1], y0 = x0 >> 8, y1 = x1 >> 8;
             const h8 va[2] = {as_h8(codes<0>(x0), codes<0>(y0), codes<0>(x1), codes<0>(y1)),
                               as_h8(codes<1>(x0), codes<1>(y0), codes<1>(x1), codes<1>(y1))};
-            uint32_t pw[4];   // keys i and i + 2 of each half
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int u = k / 2, i = k % 2;
-                const float p0 = sc[u][i], p1 = sc[u][i + 2];
-                const float d0 = half_of(cv.d[u][b][0], i), d1 = half_of(cv.d[u][b][1], i);
-                uint32_t hi = word_of((_Float16) __builtin_fmaf(p0, d0, 0.0f), (_Float16) __builtin_fmaf(p1, d1, 0.0f));
-                if (NS == 2) {
-                    // (one rounding of the product for both uses: the compiler may round it in one step or in two)
-                    asm volatile("" : "+v"(hi));
-                    const uint32_t lo = word_of((_Float16) __builtin_fmaf(p0, d0, -half_of(hi, 0)),
-                                                (_Float16) __builtin_fmaf(p1, d1, -half_of(hi, 1)));
-                    hi = m < RC ? hi : lo;
-                }
-                pw[k] = hi;
-            }
-            if (masked)   // (a masked key's scale may be a NaN)
+            {
+                uint32_t pw[4];   // keys i and i + 2 of each half
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int key = key0 + 16 * (k / 2) + k % 2;
-                    pw[k] &= (key <= see ? 0xffffu : 0u) | (key + 2 <= see ? 0xffff0000u : 0u);
+                    const int u = k / 2, i = k % 2;
+                    const float p0 = sc[u][i], p1 = sc[u][i + 2];
+                    const float d0 = half_of(vd[u][b][0], i), d1 = half_of(vd[u][b][1], i);
+                    // (one fp32 rounding of the products whatever the compiler would make of them)
+                    float w0 = __builtin_fmaf(p0, d0, 0.0f), w1 = __builtin_fmaf(p1, d1, 0.0f);
+                    asm volatile("" : "+v"(w0), "+v"(w1));
+                    uint32_t hi = word_of((_Float16) w0, (_Float16) w1);
+                    if (NS == 2) {
+                        asm volatile("" : "+v"(hi));
+                        float v0 = __builtin_fmaf(p0, d0, -half_of(hi, 0)), v1 = __builtin_fmaf(p1, d1, -half_of(hi, 1));
+                        asm volatile("" : "+v"(v0), "+v"(v1));
+                        hi = (hi & high) | (word_of((_Float16) v0, (_Float16) v1) & ~high);
+                    }
+                    pw[k] = hi;
                 }
-            const h8 pb = as_h8(pw[0], pw[1], pw[2], pw[3]);
+                if (masked)   // (a masked key's scale may be a NaN)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) o[2 * b + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[k], pb, o[2 * b + k], 0, 0, 0);
+                    for (int k = 0; k < 4; ++k) {
+                        const int key = key0 + 16 * (k / 2) + k % 2;
+                        pw[k] &= (key <= see ? 0xffffu : 0u) | (key + 2 <= see ? 0xffff0000u : 0u);
+                    }
+                const h8 pb = as_h8(pw[0], pw[1], pw[2], pw[3]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) o[2 * b + k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[k], pb, o[2 * b + k], 0, 0, 0);
+            }
         }
-        if (BUF == 1 && next < c1) nv.load(cell, l);
-        c = next;
-    };
-    while (c < c1) {
-        turn(0);
-        if (BUF == 1) continue;
-        if (c >= c1) break;
-        turn(1);
     }
 
     // the waves' sums meet in LDS
-    lsum += __shfl_xor(lsum, 16);
-    lsum += __shfl_xor(lsum, 32);
-    if (l < RC) {
-        s_off[w][l] = off;
-        s_l[w][l] = lsum;
-    }
+    lsum = sum_over_groups(lsum);
+    if (l < RC) s_ol[w][l] = float2{off, lsum};
+    if (NS == 2)
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) {
-        if (NS == 2)
+        for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] += other_part(o[i][j]);
-        if (m < RC) *(f4*) (s_o + (w * RC + m) * LD + 16 * i + 4 * g) = o[i];
-    }
-    __syncthreads();
+    __syncthreads();   // (every wave is done with its ring)
+    float* s_o = (float*) s_ring;
+    if (m < RC)
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) *(f4*) (s_o + (w * RC + m) * LD + 16 * i + 4 * g) = o[i];
     const int ways = 1 << cshift, tiles = 1 << tshift;
-    for (int e = tid; e < rows * (D / 4); e += 64 * W) {
-        const int row = e / (D / 4), dim = 4 * (e % (D / 4)), tile = row / RC, rr = row % RC;
-        float at = NO_KEY, sum = 0.0f;
-        for (int k = 0; k < ways; ++k) at = fmaxf(at, s_off[tile + tiles * k][rr]);
-        f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = 0; k < ways; ++k) {
-            const int from = tile + tiles * k;
-            const float f = exp2_hw(s_off[from][rr] - at);
-            v += *(const f4*) (s_o + (from * RC + rr) * LD + dim) * f;
-            sum += s_l[from][rr] * f;
+    __syncthreads();
+    for (int e = tid; e < rows * (D / 2); e += 64 * W) {
+        const int row = e / (D / 2), dim = 2 * (e % (D / 2)), tile = row / RC, rr = row % RC;
+        float2 ol[W], part[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const int from = tile + tiles * (k & (ways - 1));
+            ol[k] = s_ol[from][rr];
+            part[k] = *(const float2*) (s_o + (from * RC + rr) * LD + dim);
         }
-        v *= 512.0f;
-        const int tok = (int) ((unsigned) row / R), hh = hd * (int) R + (int) ((unsigned) row % R), lastc = (back + tok) >> 5;
+        float at = ol[0].x, sum = 0.0f;
+#pragma unroll
+        for (int k = 1; k < W; ++k) at = fmaxf(at, ol[k].x);
+        float2 v = float2{0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float f = k < ways ? exp2_hw(ol[k].x - at) : 0.0f;
+            v.x += k < ways ? part[k].x * f : 0.0f;   // (0 times a NaN)
+            v.y += k < ways ? part[k].y * f : 0.0f;
+            sum += k < ways ? ol[k].y * f : 0.0f;
+        }
+        const int tok = by_R(row), hh = hd * R + row - tok * R, lastc = (back + tok) >> 5;
         if (lastc < a.cells) {          // the row's keys are all in the first split
             if (z > 0) continue;
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            q4_put4((char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1, a.type, hh * D + dim, v * inv);
+            const float inv = sum == 0.0f ? 0.0f : 512.0f / sum;
+            q4_put2((char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1, a.type, hh * D + dim, v.x * inv, v.y * inv);
         } else if (zc <= lastc) {
             const int64_t p = (((int64_t) z * a.S + s.i) * a.tcap + tok) * a.n_head + hh;
-            *(f4*) (a.part + p * D + dim) = v;
+            *(float2*) (a.part + p * D + dim) = float2{v.x * 512.0f, v.y * 512.0f};
             if (dim == 0) *(float2*) (a.stat + 2 * p) = float2{at, sum};
         }
     }
@@ -622,13 +677,8 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
                     }
                 if (__any(any_nan)) nans |= 1 << k;
             }
-            auto settle = [&](uint32_t t, int& sh) {
-#pragma unroll
-                for (int k = 32; k >= 1; k >>= 1) t = max(t, (uint32_t) __shfl_xor((int) t, k));
-                sh = min(sh, uni(29 - (int) (t >> 10)));   // exponent(d) + sh <= 14
-            };
-            settle(top[0], sk);
-            settle(top[1], sv);
+            sk = min(sk, 29 - (max_of_wave((int) top[0]) >> 10));   // exponent(d) + sk <= 14
+            sv = min(sv, 29 - (max_of_wave((int) top[1]) >> 10));
         }
         const int mine = w / RN, keys = gone >> mine & 1 ? 0 : len - 32 * (c + mine);   // its cell, the request's keys in it
 #pragma unroll
@@ -691,7 +741,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         const bool ok = r < rows;
         const int t = ok ? (int) ((unsigned) r / R) : 0, h = ok ? hd * (int) R + (int) ((unsigned) r % R) : 0;
         lim[n] = ok ? back + t : -1;
-        qs[n] = 512.0f * q4_load_q<D, NS>(a, s.row0 + t, h, ok, l, q[n]);
+        Q4Row<D, NS> x;
+        x.load(a, s.row0 + t, h, l);
+        qs[n] = 512.0f * x.parts(a, ok, l, q[n]);
     }
     f4 o[NC][2 * NB];            // O^T 2^(osv - 9)
     float off[NC], mx[NC], lsum[NC];
@@ -750,9 +802,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
             for (int i = 1; i < 8; ++i) smax = fmaxf(smax, sc[n][i / 4][i % 4]);
             if (__any(__builtin_fmaf(smax, qn, -off[n]) > 12.0f)) {
-                smax = fmaxf(smax, __shfl_xor(smax, 16));
-                smax = fmaxf(smax, __shfl_xor(smax, 32));
-                mx[n] = fmaxf(mx[n], smax * qn);
+                mx[n] = fmaxf(mx[n], max_over_groups(smax) * qn);
                 const float now = mx[n] == NO_KEY ? NO_KEY : mx[n] - 4.0f, f = exp2_hw(off[n] - now);
                 off[n] = now;
                 lsum[n] *= f;
@@ -816,8 +866,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const float unit = bitsf((uint32_t) (127 + 9 - osv) << 23);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        lsum[n] += __shfl_xor(lsum[n], 16);
-        lsum[n] += __shfl_xor(lsum[n], 32);
+        lsum[n] = sum_over_groups(lsum[n]);
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
             o[n][i] *= unit;
@@ -930,8 +979,8 @@ __global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int mos
 // Requests of up to `few` rows are k_attn_q4's, the others k_attn_q4_rows' (a lone request that may have more rows: too).
 template <int D, int NS>
 int launch(const AttnQ4Args& a, hipStream_t st) {
-    constexpr int W = q4_group(D);
-    const int few = a.tcap > 0 ? W * (16 / NS) : 0;
+    constexpr int W = q4_waves(D);
+    const int few = a.tcap > 0 ? Q4_TILES * (16 / NS) : 0;
     const unsigned nk = (unsigned) a.c.n_head_kv;
     if (few) {
         hipLaunchKernelGGL((k_attn_q4<D, NS>), dim3((unsigned) a.S, nk, (unsigned) a.splits), dim3(64 * W), 0, st, a);
@@ -951,7 +1000,7 @@ int launch(const AttnQ4Args& a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 int parts_of(const AttnQ4Args& a) { return a.type == KV_F32 ? 8 : 16; }   // rows of a 16-column tile
-int few_of(const AttnQ4Args& a) { return q4_group(a.c.D) * parts_of(a); }
+int few_of(const AttnQ4Args& a) { return Q4_TILES * parts_of(a); }
 
 }  // namespace
 
@@ -962,7 +1011,12 @@ int64_t q4_few_tokens(const AttnQ4Args& a) {
 int64_t q4_splits(const AttnQ4Args& a) {
     if (q4_few_tokens(a) == 0) return 1;
     const int64_t groups = (int64_t) a.S * a.c.n_head_kv, cells = (a.max_len + KV_CELL - 1) / KV_CELL;
-    return std::max<int64_t>(1, std::min<int64_t>({512 / groups, cells / 16, 4096}));
+    const int64_t rows = q4_few_tokens(a) * (a.n_head / a.c.n_head_kv), W = q4_waves(a.c.D);
+    int64_t tiles = 1;
+    while (tiles < Q4_TILES && tiles * parts_of(a) < rows) tiles *= 2;
+    // A workgroup to a CU; twice as many for requests of one tile, which are seldom all as long as the longest
+    const int64_t want = a.S > 1 && tiles == 1 ? 512 : 256;
+    return std::max<int64_t>(1, std::min<int64_t>({want / groups, cells / (2 * (W / tiles)), 4096}));
 }
 int64_t q4_row_blocks(const AttnQ4Args& a) {
     const int per = 8 / qr_halves(a.c.D) * qr_tiles(a.c.D) * parts_of(a);

@@ -77,6 +77,8 @@ struct AttnQ4Args {
     void* out;                            // likewise
     size_t q_nb1, out_nb1;
     int n_head, S;
+    int group;                            // query heads per kv head, and 2^32 / group rounded up
+    uint32_t group_inv;
     int64_t T, W;
     const int32_t *table, *seq_start, *seq_len;
     int64_t max_new, max_len;
