@@ -21,7 +21,9 @@ def _torch():
 
 
 def stream() -> int:
-    return _torch().cuda.current_stream().cuda_stream
+    """The current device's current stream."""
+    torch = _torch()
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())   # (current_stream() builds an object: 3 us)
 
 
 def init(device: int = 0, workspace_bytes: int = 0) -> None:
@@ -475,24 +477,27 @@ def decoder_layer(attn, moe: Layer, h, n_past: int, rms_eps: float = 1e-6):
 
 def _kv_type(dtype) -> int:
     torch = _torch()
-    t = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
-    if t is None:
-        raise TypeError(f"rows of {dtype}: the cache takes float32, float16 and bfloat16")
-    return t
+    if dtype is torch.float32:
+        return F32
+    if dtype is torch.float16:
+        return F16
+    if dtype is torch.bfloat16:
+        return BF16
+    raise TypeError(f"rows of {dtype}: the cache takes float32, float16 and bfloat16")
 
 
-def _kv_rows(x, name: str, heads: int, D: int):
+def _kv_rows(x, name: str, T: int, heads: int, D: int) -> int:
     """Byte stride between the token rows of x [T, heads, D]; the heads of a token are dense."""
-    if x.dim() != 3 or tuple(x.shape[1:]) != (heads, D):
-        raise ValueError(f"{name}: [tokens, {heads}, {D}] is wanted, got {tuple(x.shape)}")
-    if x.stride(2) != 1 or (heads > 1 and x.stride(1) != D):
+    if x.shape != (T, heads, D):
+        raise ValueError(f"{name}: [{T}, {heads}, {D}] is wanted, got {tuple(x.shape)}")
+    st = x.stride()
+    if st[2] != 1 or (heads > 1 and st[1] != D):
         raise ValueError(f"{name}: the heads of a token have to be dense")
-    return x.stride(0) * x.element_size() if x.shape[0] > 1 else heads * D * x.element_size()
+    return (st[0] if T > 1 else heads * D) * x.element_size()
 
 
-def _kv_index(x, name: str, dtype, *shape):
-    if x.dtype != dtype or not x.is_contiguous() or any(n is not None and m != n for m, n in zip(x.shape, shape)) \
-            or x.dim() != len(shape):
+def _kv_index(x, name: str, dtype, *shape) -> None:
+    if x.dtype is not dtype or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{name}: dense {dtype} {shape} is wanted, got {x.dtype} {tuple(x.shape)}")
 
 
@@ -518,37 +523,39 @@ def kv_plan(held, past, new, page_tokens: int, page_table, ring, counters, n_tok
     [S, W] and ring i32 [n_pages] are updated in place; counters i64 [2] (head, tail).
     Returns (the next counters, seq_start [S + 1], seq_len [S], slot i64 [n_tokens], pos [n_tokens])."""
     torch = _torch()
+    i32, i64 = torch.int32, torch.int64
     S, W = page_table.shape
-    for x, name in ((held, "held"), (past, "past"), (new, "new")):
-        _kv_index(x, name, torch.int32, S)
-    _kv_index(page_table, "page_table", torch.int32, S, W)
-    _kv_index(ring, "ring", torch.int32, None)
-    _kv_index(counters, "counters", torch.int64, 2)
+    n_pages = ring.numel()
+    _kv_index(held, "held", i32, S)
+    _kv_index(past, "past", i32, S)
+    _kv_index(new, "new", i32, S)
+    _kv_index(page_table, "page_table", i32, S, W)
+    _kv_index(ring, "ring", i32, n_pages)
+    _kv_index(counters, "counters", i64, 2)
     dev = held.device
-    out = torch.empty(2, dtype=torch.int64, device=dev)
-    start = torch.empty(S + 1, dtype=torch.int32, device=dev)
-    length = torch.empty(S, dtype=torch.int32, device=dev)
-    slot = torch.empty(n_tokens, dtype=torch.int64, device=dev)
-    pos = torch.empty(n_tokens, dtype=torch.int32, device=dev)
-    check(lib().qwmoe_kv_plan(stream(), _ptr(held), _ptr(past), _ptr(new), S, page_tokens, ring.numel(), _ptr(page_table), W,
-                              _ptr(ring), _ptr(counters), _ptr(out), n_tokens, _ptr(start), _ptr(length), _ptr(slot),
-                              _ptr(pos)), "kv_plan")
+    wide = torch.empty(2 + n_tokens, dtype=i64, device=dev)     # one allocation per type
+    narrow = torch.empty(2 * S + 1 + n_tokens, dtype=i32, device=dev)
+    out, slot = torch.unsafe_split_with_sizes(wide, (2, n_tokens))   # (half of split()'s time)
+    start, length, pos = torch.unsafe_split_with_sizes(narrow, (S + 1, S, n_tokens))
+    p8, p4 = wide.data_ptr(), narrow.data_ptr()
+    check(lib().qwmoe_kv_plan(stream(), held.data_ptr(), past.data_ptr(), new.data_ptr(), S, page_tokens, n_pages,
+                              page_table.data_ptr(), W, ring.data_ptr(), counters.data_ptr(), p8, n_tokens, p4, p4 + 4 * (S + 1),
+                              p8 + 16, p4 + 4 * (2 * S + 1)), "kv_plan")
     return out, start, length, slot, pos
 
 
 def kv_q4_store(cache: KvQ4, k, v, slot) -> None:
     """k, v [T, n_head_kv, D] (f32, f16 or bf16; token rows may be strided) quantized into the
     cache at slot i64 [T] (negative: passed over)."""
-    torch = _torch()
-    T = k.shape[0]
-    nbk = _kv_rows(k, "k", cache.n_head_kv, cache.n_embd_head)
-    nbv = _kv_rows(v, "v", cache.n_head_kv, cache.n_embd_head)
-    if v.dtype != k.dtype or v.shape[0] != T:
-        raise ValueError("k and v: one type and one number of rows are wanted")
-    _kv_index(slot, "slot", torch.int64, T)
+    T, heads, D = k.shape[0], cache.n_head_kv, cache.n_embd_head
+    nbk = _kv_rows(k, "k", T, heads, D)
+    nbv = _kv_rows(v, "v", T, heads, D)
+    if v.dtype is not k.dtype:
+        raise ValueError("k and v: one type is wanted")
+    _kv_index(slot, "slot", _torch().int64, T)
     typ = _kv_type(k.dtype)
     if T:
-        check(lib().qwmoe_kv_q4_store(stream(), C.byref(cache), typ, _ptr(k), nbk, _ptr(v), nbv, _ptr(slot), T),
+        check(lib().qwmoe_kv_q4_store(stream(), C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
               "kv_q4_store")
 
 
@@ -556,19 +563,19 @@ def kv_q4_load(cache: KvQ4, slot, dtype=None, out=None):
     """The cache's rows at slot i64 [T]: (k, v) [T, n_head_kv, D] of ``dtype`` (f32), or into
     out = (k, v).  Rows with a negative slot are not written."""
     torch = _torch()
-    T = slot.shape[0]
+    T, heads, D = slot.shape[0], cache.n_head_kv, cache.n_embd_head
     if out is None:
-        shape = (T, cache.n_head_kv, cache.n_embd_head)
-        out = tuple(torch.empty(shape, dtype=dtype or torch.float32, device=slot.device) for _ in range(2))
-    k, v = out
-    nbk = _kv_rows(k, "k", cache.n_head_kv, cache.n_embd_head)
-    nbv = _kv_rows(v, "v", cache.n_head_kv, cache.n_embd_head)
-    if v.dtype != k.dtype or k.shape[0] != T or v.shape[0] != T:
-        raise ValueError("k and v: one type and a row per slot are wanted")
+        k, v = torch.empty((2, T, heads, D), dtype=dtype or torch.float32, device=slot.device).unbind(0)
+    else:
+        k, v = out
+    nbk = _kv_rows(k, "k", T, heads, D)
+    nbv = _kv_rows(v, "v", T, heads, D)
+    if v.dtype is not k.dtype:
+        raise ValueError("k and v: one type is wanted")
     _kv_index(slot, "slot", torch.int64, T)
     typ = _kv_type(k.dtype)
     if T:
-        check(lib().qwmoe_kv_q4_load(stream(), C.byref(cache), typ, _ptr(k), nbk, _ptr(v), nbv, _ptr(slot), T),
+        check(lib().qwmoe_kv_q4_load(stream(), C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
               "kv_q4_load")
     return k, v
 
@@ -579,21 +586,21 @@ def attn_kv_q4(cache: KvQ4, q, page_table, seq_start, seq_len, max_new: int, max
     [S + 1], seq_len i32 [S]; max_new, max_len bound the requests' new tokens and
     lengths; scale 0: 1 / sqrt(D).  Returns out; rows behind the last request are not written."""
     torch = _torch()
-    T, nq, D = q.shape
+    T, nq, D = q.shape[0], q.shape[1], cache.n_embd_head
     S, W = page_table.shape
-    nbq = _kv_rows(q, "q", nq, cache.n_embd_head)
+    nbq = _kv_rows(q, "q", T, nq, D)
     if out is None:
         out = torch.empty((T, nq, D), dtype=q.dtype, device=q.device)
-    nbo = _kv_rows(out, "out", nq, D)
-    if out.dtype != q.dtype or out.shape[0] != T:
-        raise ValueError("out: q's type and number of rows are wanted")
+    nbo = _kv_rows(out, "out", T, nq, D)
+    if out.dtype is not q.dtype:
+        raise ValueError("out: q's type is wanted")
     _kv_index(page_table, "page_table", torch.int32, S, W)
     _kv_index(seq_start, "seq_start", torch.int32, S + 1)
     _kv_index(seq_len, "seq_len", torch.int32, S)
     typ = _kv_type(q.dtype)
     if T:
-        check(lib().qwmoe_attn_kv_q4(stream(), C.byref(cache), typ, _ptr(q), nbq, nq, _ptr(page_table), W,
-                                     _ptr(seq_start), _ptr(seq_len), S, T, max_new, max_len, scale, _ptr(out), nbo),
+        check(lib().qwmoe_attn_kv_q4(stream(), C.byref(cache), typ, q.data_ptr(), nbq, nq, page_table.data_ptr(), W,
+                                     seq_start.data_ptr(), seq_len.data_ptr(), S, T, max_new, max_len, scale, out.data_ptr(), nbo),
               "attn_kv_q4")
     return out
 
