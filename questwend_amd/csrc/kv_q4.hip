@@ -20,17 +20,24 @@ namespace {
 // of the token rows, of the new table entries and of the returned pages.  A row's
 // page comes from the table where the request already held it, else from the
 // ring, so no workgroup waits for another's writes.
-struct PlanSeq {
-    int n, have, need, grow, give;   // grow: pages wanted; give: pages to put back
-    bool good;
-};
-
-__device__ __forceinline__ int64_t wave_incl(int64_t v, int lane) {
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
+// A few kilobytes: what it takes is the chain counters -> three scans -> row's search -> page -> slot,
+// so the scans stay in registers (DPP adds, one LDS exchange each).  One decode step of 24
+// requests 3.9 us, a round of 512 with 3000 tokens' prompts 6.3 (with 64-bit shuffles
+// 5.0 and 8.6); an empty kernel takes 1.4.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ uint32_t kv_dpp(uint32_t v) {
+    return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, ROWS, 0xF, true);
+}
+// Sums that stay at 2^32 - 1 once there: above every bound they are compared with (rows, pages
+// and widths are below 2^31, as is each addend, so a sum that matters is not clipped).
+__device__ __forceinline__ uint32_t kv_add(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ uint32_t kv_wave_incl(uint32_t v) {   // sums over the lanes up to this one
+    v = kv_add(v, kv_dpp<0x111>(v));
+    v = kv_add(v, kv_dpp<0x112>(v));
+    v = kv_add(v, kv_dpp<0x114>(v));
+    v = kv_add(v, kv_dpp<0x118>(v));
+    v = kv_add(v, kv_dpp<0x142, 0xA>(v));   // the last of row 0 to row 1, of row 2 to row 3
+    return kv_add(v, kv_dpp<0x143, 0xC>(v));   // the last of row 1 to rows 2 and 3
 }
 
 __global__ void __launch_bounds__(256) k_kv_plan(KvPlanArgs a) {
@@ -38,14 +45,26 @@ __global__ void __launch_bounds__(256) k_kv_plan(KvPlanArgs a) {
     int32_t* s_start = s_mem;                 // [S + 1] token rows before request i, at most T
     int32_t* s_take = s_start + a.S + 1;      // [S + 1] pages taken before request i
     int32_t* s_give = s_take + a.S + 1;       // [S + 1] pages put back before request i
-    __shared__ int64_t s_part[3][4];
+    __shared__ uint32_t s_part[4][4];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int P1 = (1 << a.page_shift) - 1;
     const int64_t head = a.counters[0], tail = a.counters[1];
-    const int64_t avail = max((int64_t) 0, min(tail - head, a.n_pages));
-    int64_t c_new = 0, c_take = 0, c_give = 0;   // sums over the requests before this round's 256
-    int64_t taken = 0;                           // pages of the served requests so far
+    const uint32_t avail = (uint32_t) max((int64_t) 0, min(tail - head, a.n_pages));
+    uint32_t c_new = 0, c_take = 0, c_give = 0;   // sums over the requests before this round's 256
+    uint32_t taken = 0;                           // pages of the served requests so far
     bool bad = false, lacking = false;
+    // the sum up to this lane over the round, on top of c; c takes the round's
+    auto scan = [&](uint32_t v, uint32_t& c, uint32_t* part) {
+        v = kv_wave_incl(v);
+        if (lane == 63) part[w] = v;
+        __syncthreads();
+        uint32_t before = c;
+        for (int u = 0; u < 4; ++u) {
+            if (u < w) before = kv_add(before, part[u]);
+            c = kv_add(c, part[u]);
+        }
+        return kv_add(before, v);
+    };
     for (int base = 0; base < a.S; base += 256) {
         const int i = base + tid;
         int held = 0, past = 0, nn = 0;
@@ -54,32 +73,22 @@ __global__ void __launch_bounds__(256) k_kv_plan(KvPlanArgs a) {
             past = a.past[i];
             nn = a.n_new[i];
         }
-        const int64_t n = max(nn, 0);
+        const uint32_t n = (uint32_t) max(nn, 0);
         const int64_t have = ((int64_t) held + P1) >> a.page_shift, need = ((int64_t) past + n + P1) >> a.page_shift;
         const bool sane = held >= 0 && past >= 0 && past <= held && nn >= 0 && have <= a.W && need <= a.W;
         // start, and whether the rows fit
-        int64_t v0 = wave_incl(n, lane);
-        if (lane == 63) s_part[0][w] = v0;
-        __syncthreads();
-        for (int u = 0; u < w; ++u) v0 += s_part[0][u];
-        const int64_t end = c_new + v0;
-        const bool good = i < a.S && sane && end <= a.T;
-        int64_t v1 = wave_incl(good ? max(need - have, (int64_t) 0) : 0, lane);
-        if (lane == 63) s_part[1][w] = v1;
-        __syncthreads();
-        for (int u = 0; u < w; ++u) v1 += s_part[1][u];
-        const int64_t upto = c_take + v1, grow = good ? max(need - have, (int64_t) 0) : 0;
+        const uint32_t end = scan(n, c_new, s_part[0]);
+        const bool good = i < a.S && sane && end <= (uint32_t) a.T;
+        const uint32_t grow = good ? (uint32_t) max(need - have, (int64_t) 0) : 0;
+        const uint32_t upto = scan(grow, c_take, s_part[1]);
         const bool served = good && (grow == 0 || upto <= avail);
-        int64_t v2 = wave_incl(served ? max(have - need, (int64_t) 0) : 0, lane);
-        if (lane == 63) s_part[2][w] = v2;
-        __syncthreads();
-        for (int u = 0; u < w; ++u) v2 += s_part[2][u];
-        const int64_t give = served ? max(have - need, (int64_t) 0) : 0;
+        const uint32_t give = served ? (uint32_t) max(have - need, (int64_t) 0) : 0;
+        const uint32_t back = scan(give, c_give, s_part[2]);
         if (i < a.S) {
-            s_start[i] = (int32_t) min(end - n, a.T);
+            s_start[i] = (int32_t) min(end - n, (uint32_t) a.T);
             // (a request that is not served: marked by the sign, its prefix is not used)
-            s_take[i] = served ? (int32_t) min(upto - grow, a.n_pages) : -1;
-            s_give[i] = (int32_t) min(c_give + v2 - give, a.n_pages);
+            s_take[i] = served ? (int32_t) min(upto - grow, (uint32_t) a.n_pages) : -1;
+            s_give[i] = (int32_t) min(back - give, (uint32_t) a.n_pages);
             if (blockIdx.x == 0) {
                 a.seq_start[i] = s_start[i];
                 a.seq_len[i] = served ? (int32_t) (past + n) : 0;
@@ -87,21 +96,22 @@ __global__ void __launch_bounds__(256) k_kv_plan(KvPlanArgs a) {
             bad |= !good;
             lacking |= good && !served;
         }
-        c_new += s_part[0][0] + s_part[0][1] + s_part[0][2] + s_part[0][3];
-        c_take += s_part[1][0] + s_part[1][1] + s_part[1][2] + s_part[1][3];
-        c_give += s_part[2][0] + s_part[2][1] + s_part[2][2] + s_part[2][3];
         // the largest prefix within avail (prefixes ascend, so the served requests' last)
-        int64_t t = served && grow > 0 ? upto : 0;
-        for (int o = 32; o >= 1; o >>= 1) t = max(t, (int64_t) __shfl_xor(t, o));
+        uint32_t t = served && grow > 0 ? upto : 0;
+        t = max(t, kv_dpp<0x111>(t));
+        t = max(t, kv_dpp<0x112>(t));
+        t = max(t, kv_dpp<0x114>(t));
+        t = max(t, kv_dpp<0x118>(t));
+        t = max(t, kv_dpp<0x142, 0xA>(t));
+        t = max(t, kv_dpp<0x143, 0xC>(t));
+        if (lane == 63) s_part[3][w] = t;
         __syncthreads();
-        if (lane == 0) s_part[0][w] = t;
-        __syncthreads();
-        taken = max(max(taken, max(s_part[0][0], s_part[0][1])), max(s_part[0][2], s_part[0][3]));
-        __syncthreads();
+        for (int u = 0; u < 4; ++u) taken = max(taken, s_part[3][u]);
+        // (the next round writes s_part[0] while slower waves still read s_part[3]: others' words)
     }
-    const int64_t given = min(c_give, a.n_pages);
+    const uint32_t given = min(c_give, (uint32_t) a.n_pages);
     if (tid == 0) {
-        s_start[a.S] = (int32_t) min(c_new, a.T);
+        s_start[a.S] = (int32_t) min(c_new, (uint32_t) a.T);
         s_take[a.S] = (int32_t) taken;
         s_give[a.S] = (int32_t) given;
         if (blockIdx.x == 0) {
@@ -201,10 +211,6 @@ __device__ __forceinline__ void kv_put4(char* row, int n, const float (&x)[4]) {
     }
 }
 
-template <int CTRL>
-__device__ __forceinline__ uint32_t kv_dpp(uint32_t v) {
-    return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, 0xF, 0xF, true);
-}
 // Ordered by magnitude, the positive one of two above the negative; 0xff000000 and up: not finite.
 __device__ __forceinline__ uint32_t kv_rank(float x) {
     const uint32_t v = fbits(x);
