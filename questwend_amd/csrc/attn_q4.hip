@@ -207,7 +207,7 @@ struct Q4Row {
 #pragma unroll
             for (int e = 0; e < NS; ++e) x[b][e] = *(const u32x4*) (src + 64 * NS * b + 16 * e);
     }
-    __device__ __forceinline__ float parts(const AttnQ4Args& a, bool ok, int l, h8 (&q)[NB]) const {
+    __device__ __forceinline__ float parts(const AttnQ4Args& a, bool ok, h8 (&q)[NS][NB]) const {
         const bool f16 = a.type == KV_F16;
         auto value = [&](int b, int j) {
             if constexpr (NS == 2) return bitsf(x[b][j / 4][j % 4]);
@@ -225,18 +225,15 @@ struct Q4Row {
         const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint32_t w[4];
+            uint32_t w[NS][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float y0 = value(b, 2 * j) * up, y1 = value(b, 2 * j + 1) * up;
-                w[j] = word_of((_Float16) y0, (_Float16) y1);
-                if (NS == 2) {
-                    const uint32_t lo = word_of((_Float16) (y0 - half_of(w[j], 0)), (_Float16) (y1 - half_of(w[j], 1)));
-                    w[j] = (l & 8) ? lo : w[j];
-                }
-                w[j] = ok ? w[j] : 0u;
+                w[0][j] = word_of((_Float16) y0, (_Float16) y1);
+                if (NS == 2) w[NS - 1][j] = word_of((_Float16) (y0 - half_of(w[0][j], 0)), (_Float16) (y1 - half_of(w[0][j], 1)));
             }
-            q[b] = as_h8(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int e = 0; e < NS; ++e) q[e][b] = ok ? as_h8(w[e][0], w[e][1], w[e][2], w[e][3]) : as_h8(0, 0, 0, 0);
         }
         return a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
     }
@@ -560,7 +557,7 @@ __device__ __forceinline__ uint32_t pow2_h2(int e) {   // 2^e in both halves, -1
 
 template <int D, int NS, bool EXACT>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) k_attn_q4_rows(AttnQ4Args a, int most) {
-    constexpr int NB = D / 32, RC = 16 / NS, NC = qr_tiles(D), KH = qr_halves(D), RG = 8 / KH, RW = NC * RC, RB = RG * RW;
+    constexpr int NB = D / 32, RC = 16, NC = qr_tiles(D), KH = qr_halves(D), RG = 8 / KH, RW = NC * RC, RB = RG * RW;
     constexpr int RN = 8 / KH, PF = 2 * NB / RN;                // waves that form a cell's operands, K (and V) operands of each
     constexpr int PARTS = EXACT ? 2 : 1, FR = 4 * NB;           // a cell: FR operands of 64 lanes x 16 bytes per part
     __shared__ __align__(16) uint8_t s_mem[2 * KH * PARTS * FR * 1024];
@@ -596,10 +593,15 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const uint8_t* head = a.c.data + hd * a.c.head_bytes();
     const int64_t page_bytes = a.c.page_bytes();
     // pages of 64 cells at a time, one per lane
-    int pg = 0, pg_at = zc;
-    auto fetch_pages = [&](int c) {
-        pg_at = c;
-        pg = c + l < cend ? pages[(c + l) >> cpp] : 0;
+    int pg_at = zc, pg = zc + l < cend ? pages[(zc + l) >> cpp] : 0;
+    // this lane's rows, asked for together with the first pages
+    Q4Row<D, NS> qx[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const int r = min(r0 + n * RC + m, rows - 1);
+        qx[n].load(a, s.row0 + (int) ((unsigned) r / R), hd * (int) R + (int) ((unsigned) r % R), l);
+    }
+    auto check_pages = [&] {
         if (pg < 0 || pg >= a.c.n_pages) {
             atomicOr(a.status, QWMOE_STATUS_BAD_SLOT);
             pg = -1;
@@ -613,7 +615,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int vb = role * PF / 2;                               // its V operands: block vb (with one operand: half role % 2)
     auto load = [&](int step) __attribute__((always_inline)) {
         const int c = zc + step * KH;
-        if (c + KH - 1 - pg_at >= 64) fetch_pages(c);
+        if (c + KH - 1 - pg_at >= 64) {
+            pg_at = c;
+            pg = c + l < cend ? pages[(c + l) >> cpp] : 0;
+            check_pages();
+        }
 #pragma unroll
         for (int k = 0; k < KH; ++k) {
             const int ck = min(c + k, cend - 1);
@@ -727,23 +733,20 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
     };
     if (steps > 0) {
-        fetch_pages(zc);
+        check_pages();
         load(0);
     }
 
     // this lane's rows
     int lim[NC];
-    h8 q[NC][NB];
+    h8 q[NC][NS][NB];
     float qs[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        const int r = r0 + n * RC + (m & (RC - 1));
+        const int r = r0 + n * RC + m;
         const bool ok = r < rows;
-        const int t = ok ? (int) ((unsigned) r / R) : 0, h = ok ? hd * (int) R + (int) ((unsigned) r % R) : 0;
-        lim[n] = ok ? back + t : -1;
-        Q4Row<D, NS> x;
-        x.load(a, s.row0 + t, h, l);
-        qs[n] = 512.0f * x.parts(a, ok, l, q[n]);
+        lim[n] = ok ? back + (int) ((unsigned) r / R) : -1;
+        qs[n] = 512.0f * qx[n].parts(a, ok, q[n]);
     }
     f4 o[NC][2 * NB];            // O^T 2^(osv - 9)
     float off[NC], mx[NC], lsum[NC];
@@ -767,17 +770,30 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         f4 sc[NC][2];
 #pragma unroll
         for (int n = 0; n < NC; ++n) sc[n][0] = sc[n][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        // (products that add to one register stand four apart)
+        // Two operands a turn, the next turn's read ahead of this one's products; products that add to one
+        // register stand 2 NC apart.
+        constexpr int TURNS = NB * PARTS;
+        auto read2 = [&](int f, int stride, int part, h8 (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int u = 0; u < 2; ++u) x[u] = *(const h8*) operand(buf, kh, part, f + u * stride);
+        };
+        h8 x[2][2];
+        read2(0, NB, 0, x[0]);
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
+        for (int i = 0; i < TURNS; ++i) {
+            if (i + 1 < TURNS) read2((i + 1) / PARTS, NB, (i + 1) % PARTS, x[(i + 1) & 1]);
+            else read2(2 * NB, 1, 0, x[(i + 1) & 1]);   // (the values' first)
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const h8 ka = *(const h8*) operand(buf, kh, p, u * NB + b);
+            for (int e = 0; e < NS; ++e)
 #pragma unroll
-                    for (int n = 0; n < NC; ++n) sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[n][b], sc[n][u], 0, 0, 0);
-                }
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int n = 0; n < NC; ++n)
+                        if (i % PARTS + e < 2)
+                            sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i & 1][u], q[n][e][i / PARTS], sc[n][u], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         const float unit = bitsf((uint32_t) (127 - csk) << 23);
         if (csv != osv) {
             const float f = bitsf((uint32_t) (127 + csv - osv) << 23);
@@ -787,13 +803,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) o[n][i] *= f;
         }
-        u32x4 pw[NC];
+        u32x4 pw[NC][NS];
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const float qn = qs[n] * unit;
-            if (NS == 2)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sc[n][i / 4][i % 4] += other_part(sc[n][i / 4][i % 4]);
             if (masked)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -818,25 +831,28 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
             for (int k = 0; k < 4; ++k) {   // keys i and i + 2 of each half
                 const float p0 = p[4 * (k / 2) + k % 2], p1 = p[4 * (k / 2) + k % 2 + 2];
-                uint32_t hi = word_of((_Float16) p0, (_Float16) p1);
-                if (NS == 2) {
-                    const uint32_t lo = word_of((_Float16) (p0 - half_of(hi, 0)), (_Float16) (p1 - half_of(hi, 1)));
-                    hi = m < RC ? hi : lo;
-                }
-                pw[n][k] = hi;
+                const uint32_t hi = word_of((_Float16) p0, (_Float16) p1);
+                pw[n][0][k] = hi;
+                if (NS == 2) pw[n][NS - 1][k] = word_of((_Float16) (p0 - half_of(hi, 0)), (_Float16) (p1 - half_of(hi, 1)));
             }
         }
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int i = 0; i < TURNS; ++i) {
+            const int at = TURNS + i;
+            if (i + 1 < TURNS) read2(2 * NB + 2 * ((i + 1) / PARTS), 1, (i + 1) % PARTS, x[(at + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
+            for (int e = 0; e < NS; ++e)
 #pragma unroll
-                for (int f = 2 * b; f < 2 * b + 2; ++f) {
-                    const h8 va = *(const h8*) operand(buf, kh, p, 2 * NB + f);
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int n = 0; n < NC; ++n)
-                        o[n][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, as_h8(pw[n][0], pw[n][1], pw[n][2], pw[n][3]), o[n][f], 0, 0, 0);
-                }
+                        if (i % PARTS + e < 2) {
+                            f4& d = o[n][2 * (i / PARTS) + u];
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[at & 1][u], as_h8(pw[n][e][0], pw[n][e][1], pw[n][e][2], pw[n][e][3]), d, 0, 0, 0);
+                        }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (nan_here) {
             const uint8_t* cell = head + (int64_t) pages[c >> cpp] * page_bytes + (c & ((1 << cpp) - 1)) * (36 * D);
             for (int t = 0; t < 32; ++t)
@@ -860,7 +876,11 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
         lds_barrier();   // this step's operands are there; the other buffer's readers are done
         // one of a SIMD's two waves forms operands while the other multiplies
         if (w < 4) ahead(step);
-        if (work) multiply(buf, c, csk, csv, nan_here);
+        if (work) {
+            __builtin_amdgcn_s_setprio(1);
+            multiply(buf, c, csk, csv, nan_here);
+            __builtin_amdgcn_s_setprio(0);
+        }
         if (w >= 4) ahead(step);
     }
     const float unit = bitsf((uint32_t) (127 + 9 - osv) << 23);
@@ -870,9 +890,6 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
             o[n][i] *= unit;
-            if (NS == 2)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][i][j] += other_part(o[n][i][j]);
         }
     }
     if constexpr (KH == 2) {   // the second half's sums to the first
@@ -901,7 +918,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         const int r = r0 + n * RC + m;
-        if (m >= RC || r >= rows) continue;
+        if (r >= rows) continue;
         const int tok = (int) ((unsigned) r / R), h = hd * (int) R + (int) ((unsigned) r % R), lastc = (back + tok) >> 5;
         if (lastc < a.row_cells) {   // the row's keys are all in the first split
             if (z > 0) continue;
@@ -918,6 +935,23 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
 }
 
+// Four dims of a row's sum so far: of the weights 2^(s - at) and of their products.
+struct Q4Sum {
+    f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float at = NO_KEY, sum = 0.0f;
+    __device__ __forceinline__ void add(const f4& pv, float pat, float psum) {
+        const float now = fmaxf(at, pat), f0 = exp2_hw(at - now), f1 = exp2_hw(pat - now);
+        v = v * f0 + pv * f1;
+        sum = sum * f0 + psum * f1;
+        at = now;
+    }
+    __device__ __forceinline__ void add(const float* part, const float* stat, int64_t p, int D, int dim) {
+        const float2 st = *(const float2*) (stat + 2 * p);
+        add(*(const f4*) (part + p * D + dim), st.x, st.y);
+    }
+    __device__ __forceinline__ f4 value() const { return v * (sum == 0.0f ? 0.0f : 1.0f / sum); }
+};
+
 // A row's splits, joined: a workgroup per row, D / 4 lanes per split; each lane adds every
 // WAYS-th split in order, then the ways are added in order.
 template <int D>
@@ -927,30 +961,18 @@ __device__ __forceinline__ void q4_join(const AttnQ4Args& a, int tok, int h, int
     __shared__ __align__(16) f4 s_v[256];
     __shared__ float s_at[WAYS], s_sum[WAYS];
     const int tid = threadIdx.x, way = tid / LN, dim = 4 * (tid % LN);
-    f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    float at = NO_KEY, sum = 0.0f;
-    auto add = [&](const f4& pv, float pat, float psum) __attribute__((always_inline)) {
-        const float now = fmaxf(at, pat), f0 = exp2_hw(at - now), f1 = exp2_hw(pat - now);
-        v = v * f0 + pv * f1;
-        sum = sum * f0 + psum * f1;
-        at = now;
-    };
+    Q4Sum v;
 #pragma unroll 4
-    for (int z = way; z < parts; z += WAYS) {
-        const int64_t p = z * heads + row;
-        const float2 st = *(const float2*) (stat + 2 * p);
-        add(*(const f4*) (part + p * D + dim), st.x, st.y);
-    }
-    s_v[tid] = v;
+    for (int z = way; z < parts; z += WAYS) v.add(part, stat, z * heads + row, D, dim);
+    s_v[tid] = v.v;
     if (dim == 0) {
-        s_at[way] = at;
-        s_sum[way] = sum;
+        s_at[way] = v.at;
+        s_sum[way] = v.sum;
     }
     __syncthreads();
     if (way > 0) return;
-    for (int k = 1; k < WAYS; ++k) add(s_v[k * LN + tid], s_at[k], s_sum[k]);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    q4_put4((char*) a.out + (int64_t) tok * a.out_nb1, a.type, h * D + dim, v * inv);
+    for (int k = 1; k < WAYS; ++k) v.add(s_v[k * LN + tid], s_at[k], s_sum[k]);
+    q4_put4((char*) a.out + (int64_t) tok * a.out_nb1, a.type, h * D + dim, v.value());
 }
 __device__ __forceinline__ int q4_parts(int lim, int64_t cells) { return lim < 0 ? 1 : (int) ((unsigned) (lim >> 5) / (unsigned) cells) + 1; }
 
@@ -964,16 +986,23 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a, int most) {
     if (parts > 1)
         q4_join<D>(a, s.row0 + t, h, parts, a.part, a.stat, ((int64_t) s.i * a.tcap + t) * a.n_head + h, (int64_t) a.S * a.tcap * a.n_head);
 }
-// of k_attn_q4_rows: workgroups (token row, head)
+// of k_attn_q4_rows: workgroups (token row, 1024 / D heads), D / 4 lanes a row: there are rows
+// enough, so each lane adds its splits in order (a workgroup per row as above: 18.9 us for two
+// splits of 16384 rows of 128, so TODO).
 template <int D>
 __global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int most) {
+    constexpr int LN = D / 4;
     Q4Seq s;
-    const int h = blockIdx.y, tok = blockIdx.x;
-    if (!q4_find(a, threadIdx.x & 63, tok, [](int t, int) { return (int64_t) t; }, s)) return;
+    const int tid = threadIdx.x, tok = blockIdx.x, h = blockIdx.y * (256 / LN) + tid / LN, dim = 4 * (tid % LN);
+    if (!q4_find(a, tid & 63, tok, [](int t, int) { return (int64_t) t; }, s)) return;
     if (tok >= s.row0 + s.n || !q4_fits(a, s) || (int64_t) s.n * (a.n_head / a.c.n_head_kv) <= most) return;
     const int parts = q4_parts(s.len - s.n + (tok - s.row0), a.row_cells);
-    if (parts > 1)
-        q4_join<D>(a, tok, h, parts, a.row_part, a.row_stat, (int64_t) tok * a.n_head + h, a.T * a.n_head);
+    if (parts == 1 || h >= a.n_head) return;
+    const int64_t row = (int64_t) tok * a.n_head + h, rows = a.T * a.n_head;
+    Q4Sum v;
+#pragma unroll 2
+    for (int z = 0; z < parts; ++z) v.add(a.row_part, a.row_stat, z * rows + row, D, dim);
+    q4_put4((char*) a.out + (int64_t) tok * a.out_nb1, a.type, h * D + dim, v.value());
 }
 
 // Requests of up to `few` rows are k_attn_q4's, the others k_attn_q4_rows' (a lone request that may have more rows: too).
@@ -995,7 +1024,7 @@ int launch(const AttnQ4Args& a, hipStream_t st) {
             if constexpr (NS == 1) hipLaunchKernelGGL((k_attn_q4_rows<D, 1, false>), g, dim3(512), 0, st, a, few);
         } else hipLaunchKernelGGL((k_attn_q4_rows<D, NS, true>), g, dim3(512), 0, st, a, few);
         if (a.row_splits > 1)
-            hipLaunchKernelGGL(k_attn_q4_rows_join<D>, dim3((unsigned) a.T, (unsigned) a.n_head), dim3(256), 0, st, a, few);
+            hipLaunchKernelGGL(k_attn_q4_rows_join<D>, dim3((unsigned) a.T, (unsigned) ((a.n_head * (D / 4) + 255) / 256)), dim3(256), 0, st, a, few);
     }
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }
@@ -1019,13 +1048,13 @@ int64_t q4_splits(const AttnQ4Args& a) {
     return std::max<int64_t>(1, std::min<int64_t>({want / groups, cells / (2 * (W / tiles)), 4096}));
 }
 int64_t q4_row_blocks(const AttnQ4Args& a) {
-    const int per = 8 / qr_halves(a.c.D) * qr_tiles(a.c.D) * parts_of(a);
+    const int per = 8 / qr_halves(a.c.D) * qr_tiles(a.c.D) * 16;
     return a.T * (a.n_head / a.c.n_head_kv) / per + a.S;
 }
 int64_t q4_row_splits(const AttnQ4Args& a) {
     if (std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) <= few_of(a)) return 1;
     const int64_t groups = q4_row_blocks(a) * a.c.n_head_kv, cells = (a.max_len + KV_CELL - 1) / KV_CELL;
-    return std::max<int64_t>(1, std::min<int64_t>(256 / groups, cells / 16));
+    return std::max<int64_t>(1, std::min<int64_t>((256 + groups / 2) / groups, cells / 8));
 }
 
 int launch_attn_q4(const AttnQ4Args& a, hipStream_t st) {
