@@ -130,6 +130,14 @@ __device__ __forceinline__ float half_of(uint32_t w, int hi) {
     __builtin_memcpy(&x, &w, 4);
     return (float) x[hi];
 }
+// v less the low or high half of w, in one instruction
+template <int HIGH>
+__device__ __forceinline__ float less_half(float v, uint32_t w) {
+    float r;
+    if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(v));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(v));
+    return r;
+}
 __device__ __forceinline__ uint32_t word_of(_Float16 lo, _Float16 hi) {
     const h2 x = {lo, hi};
     uint32_t w;
@@ -811,21 +819,27 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     sc[n][i / 4][i % 4] = key0 + 16 * (i / 4) + i % 4 <= lim[n] ? sc[n][i / 4][i % 4] : -INFINITY;
-            float smax = sc[n][0][0];
+            float p[8], most = -INFINITY;
 #pragma unroll
-            for (int i = 1; i < 8; ++i) smax = fmaxf(smax, sc[n][i / 4][i % 4]);
-            if (__any(__builtin_fmaf(smax, qn, -off[n]) > 12.0f)) {
+            for (int i = 0; i < 8; ++i) p[i] = __builtin_fmaf(sc[n][i / 4][i % 4], qn, -off[n]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
+            if (__any(most > 12.0f)) {
+                float smax = sc[n][0][0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) smax = fmaxf(smax, sc[n][i / 4][i % 4]);
                 mx[n] = fmaxf(mx[n], max_over_groups(smax) * qn);
                 const float now = mx[n] == NO_KEY ? NO_KEY : mx[n] - 4.0f, f = exp2_hw(off[n] - now);
                 off[n] = now;
                 lsum[n] *= f;
 #pragma unroll
                 for (int i = 0; i < 2 * NB; ++i) o[n][i] *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[i] = __builtin_fmaf(sc[n][i / 4][i % 4], qn, -off[n]);
             }
-            float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                p[i] = exp2_hw(__builtin_fmaf(sc[n][i / 4][i % 4], qn, -off[n]));
+                p[i] = exp2_hw(p[i]);
                 lsum[n] += p[i];
             }
 #pragma unroll
@@ -833,7 +847,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
                 const float p0 = p[4 * (k / 2) + k % 2], p1 = p[4 * (k / 2) + k % 2 + 2];
                 const uint32_t hi = word_of((_Float16) p0, (_Float16) p1);
                 pw[n][0][k] = hi;
-                if (NS == 2) pw[n][NS - 1][k] = word_of((_Float16) (p0 - half_of(hi, 0)), (_Float16) (p1 - half_of(hi, 1)));
+                if (NS == 2) pw[n][NS - 1][k] = word_of((_Float16) less_half<0>(p0, hi), (_Float16) less_half<1>(p1, hi));
             }
         }
 #pragma unroll
@@ -987,8 +1001,8 @@ __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a, int most) {
         q4_join<D>(a, s.row0 + t, h, parts, a.part, a.stat, ((int64_t) s.i * a.tcap + t) * a.n_head + h, (int64_t) a.S * a.tcap * a.n_head);
 }
 // of k_attn_q4_rows: workgroups (token row, 1024 / D heads), D / 4 lanes a row: there are rows
-// enough, so each lane adds its splits in order (a workgroup per row as above: 18.9 us for two
-// splits of 16384 rows of 128, so TODO).
+// enough, so each lane adds its splits in order (two splits of 16384 rows of 128: 5.8 us; a
+// workgroup per row as above 18.9).
 template <int D>
 __global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int most) {
     constexpr int LN = D / 4;
