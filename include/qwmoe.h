@@ -587,7 +587,8 @@ int qwmoe_kv_q4_load(void * stream, const qwmoe_kv_q4 * cache, int type, void * 
  * (all in the cache by then); row t's head h attends to keys 0 .. seq_len - n + t of kv head
  * h / (n_head / n_head_kv):  out = sum_j softmax_j(kq_scale q . k_j) v_j.
  *   q, out: `type` (F32, F16, BF16) [n_tokens][n_head][D], tokens q_nb1 / out_nb1 bytes
- *   apart, 16-byte aligned, not the same buffer; kq_scale > 0, or 0 for 1 / sqrt(D)
+ *   apart, 16-byte aligned, not the same buffer; kq_scale 2^-20 .. 2^20, or 0 for 1 / sqrt(D)
+ *   (the scores and |q| kq_scale have to stay below 2^100)
  *   max_new, max_len: upper bounds of n and of seq_len (they size the launch: a
  *   captured call keeps them); max_len <= table_width * page_tokens < 2^31
  * A row that sees no key (seq_len 0, or n > seq_len) gets zeros; rows from
@@ -595,10 +596,16 @@ int qwmoe_kv_q4_load(void * stream, const qwmoe_kv_q4 * cache, int type, void * 
  * (QWMOE_STATUS_BAD_SEQ); keys of a page outside the pool count as masked
  * (QWMOE_STATUS_BAD_SLOT).  Sums, the softmax's statistics and the products with f32 rows are
  * in 32 bits (f32 rows enter the matrix cores as two f16 parts each); for F16 and BF16
- * rows the unnormalized weights are rounded to f16 before the sum over the values.  The
- * order of the sums follows max_new, max_len, n_seq and n_tokens, never the run.
- * Workspace where the keys are split over workgroups (few rows, long max_len): per split
- * n_tokens * n_head * (D + 2) floats, as many splits as fit. */
+ * rows the unnormalized weights are rounded to f16 before the sum over the values, and BF16
+ * requests of more than 128 rows (n * n_head / n_head_kv) have their keys and values rounded to
+ * f16 first.  A NaN or an infinity that was stored shows in the rows that see its
+ * block, in no other.  The order of the sums follows max_new, max_len, n_seq, n_tokens and
+ * the workspace's size, never the run.
+ * Workspace where the keys are split over workgroups, as many splits as fit: per split n_seq *
+ * min(max_new, n_tokens, f / (n_head / n_head_kv)) * n_head * (D + 2) floats for requests of up to
+ * f rows (64 for F32, else 128), n_tokens * n_head * (D + 2) where there may be longer ones.  A
+ * captured call keeps its place in the workspace: no two such calls run at once, and none
+ * after a qwmoe_shutdown or a qwmoe_init that enlarges it. */
 int qwmoe_attn_kv_q4(void * stream, const qwmoe_kv_q4 * cache, int type, const void * q, size_t q_nb1,
                      int64_t n_head, const int32_t * page_table, int64_t table_width, const int32_t * seq_start,
                      const int32_t * seq_len, int64_t n_seq, int64_t n_tokens, int64_t max_new, int64_t max_len,

@@ -1108,7 +1108,7 @@ int qwmoe_attn_kv_q4(void* stream, const qwmoe_kv_q4* cache, int type, const voi
         !(kq_scale < INFINITY))
         return QWMOE_ERR_INVALID_ARG;
     if (n_seq > qw::KV_MAX_SEQ || n_head > 65535 || n_tokens > 0x7fffffff / n_head ||
-        table_width > (0x7fffffff >> a.c.page_shift))
+        table_width > (0x7fffffff >> a.c.page_shift) || (kq_scale > 0.0f && (kq_scale < 0x1p-20f || kq_scale > 0x1p20f)))
         return QWMOE_ERR_UNSUPPORTED;
     if (max_len > table_width * cache->page_tokens) return QWMOE_ERR_INVALID_ARG;
     if ((rc = kv_rows(q, q_nb1, n_head * D, size)) || (rc = kv_rows(out, out_nb1, n_head * D, size))) return rc;

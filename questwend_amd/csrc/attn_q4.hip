@@ -229,7 +229,7 @@ struct Q4Row {
             for (int j = 0; j < 8; ++j) big = fmaxf(big, __builtin_fabsf(value(b, j)));
         big = max_over_groups(big);
         // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
-        const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
+        const int ex = min(max((int) (fbits(big) >> 23) - 127, -60), 127);
         const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
         }
         big = max_over_groups(max_over_16(big));
         // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
-        const int ex = min(max((int) (fbits(big) >> 23) - 127, -100), 100);
+        const int ex = min(max((int) (fbits(big) >> 23) - 127, -60), 127);
         const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
         _Float16* dst = s_q + i * LQ + E * l;
 #pragma unroll

@@ -486,6 +486,13 @@ def _kv_type(dtype) -> int:
     raise TypeError(f"rows of {dtype}: the cache takes float32, float16 and bfloat16")
 
 
+def _kv_here(*tensors) -> None:
+    dev = _torch().cuda.current_device()
+    for x in tensors:
+        if x.get_device() != dev:   # (-1: host memory)
+            raise ValueError(f"tensors of the current device (cuda:{dev}) are wanted, got one of {x.device}")
+
+
 def _kv_rows(x, name: str, T: int, heads: int, D: int) -> int:
     """Byte stride between the token rows of x [T, heads, D]; the heads of a token are dense."""
     if x.shape != (T, heads, D):
@@ -532,6 +539,7 @@ def kv_plan(held, past, new, page_tokens: int, page_table, ring, counters, n_tok
     _kv_index(page_table, "page_table", i32, S, W)
     _kv_index(ring, "ring", i32, n_pages)
     _kv_index(counters, "counters", i64, 2)
+    _kv_here(held, past, new, page_table, ring, counters)
     dev = held.device
     wide = torch.empty(2 + n_tokens, dtype=i64, device=dev)     # one allocation per type
     narrow = torch.empty(2 * S + 1 + n_tokens, dtype=i32, device=dev)
@@ -555,6 +563,7 @@ def kv_q4_store(cache: KvQ4, k, v, slot) -> None:
     _kv_index(slot, "slot", _torch().int64, T)
     typ = _kv_type(k.dtype)
     if T:
+        _kv_here(k, v, slot)
         check(lib().qwmoe_kv_q4_store(stream(), C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
               "kv_q4_store")
 
@@ -575,6 +584,7 @@ def kv_q4_load(cache: KvQ4, slot, dtype=None, out=None):
     _kv_index(slot, "slot", torch.int64, T)
     typ = _kv_type(k.dtype)
     if T:
+        _kv_here(k, v, slot)
         check(lib().qwmoe_kv_q4_load(stream(), C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
               "kv_q4_load")
     return k, v
@@ -599,6 +609,7 @@ def attn_kv_q4(cache: KvQ4, q, page_table, seq_start, seq_len, max_new: int, max
     _kv_index(seq_len, "seq_len", torch.int32, S)
     typ = _kv_type(q.dtype)
     if T:
+        _kv_here(q, out, page_table, seq_start, seq_len)
         check(lib().qwmoe_attn_kv_q4(stream(), C.byref(cache), typ, q.data_ptr(), nbq, nq, page_table.data_ptr(), W,
                                      seq_start.data_ptr(), seq_len.data_ptr(), S, T, max_new, max_len, scale, out.data_ptr(), nbo),
               "attn_kv_q4")

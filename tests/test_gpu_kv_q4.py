@@ -606,3 +606,133 @@ def test_same_call_twice_gives_the_same_bits():
     first = b.run()
     for _ in range(5):
         assert torch.equal(b.run(), first)
+
+
+# ---- requests of many rows: the keys split over workgroups -----------------------------
+
+
+MANY = [(128, 1, 8, 64), (64, 2, 14, 128), (256, 1, 8, 32), (128, 2, 2, 256)]
+
+
+@pytest.mark.parametrize("typ", list(TYPES))
+@pytest.mark.parametrize("D,heads,Hq,P", MANY)
+@pytest.mark.parametrize("lens,new", [([3000], [140]), ([2500, 700, 60], [150, 1, 3]), ([129, 1900], [129, 200])])
+def test_many_rows_over_splits(typ, D, heads, Hq, P, lens, new):
+    b = Batch(60 + D, heads, D, P, lens, new, typ, Hq, pad=3)
+    out = torch.full_like(b.q, 5.0)
+    b.run(out=out)
+    b.check(out)
+    assert torch.equal(out[b.start[-1]:], torch.full_like(out[b.start[-1]:], 5.0))
+    b.check(b.run(max_new=max(new) + 77, max_len=b.table.shape[1] * P))       # wider bounds: other splits
+    assert status() == 0
+
+
+@pytest.mark.parametrize("typ", list(TYPES))
+@pytest.mark.parametrize("D,heads,Hq,P", MANY)
+def test_many_rows_bad_pages_and_nans(typ, D, heads, Hq, P):
+    """A page outside the pool in the middle of the keys, and a NaN and an infinity that only the last row sees."""
+    n, new = 2000, 150
+    b = Batch(61, heads, D, P, [n], [new], typ, Hq)
+    keep, at = b.table.copy(), 1000 // P
+    b.table[0, at] = b.cache.n_pages
+    got = b.run()
+    assert status() == qa.STATUS_BAD_SLOT
+    k, v = b.k64[0], b.v64[0]
+    seen = np.r_[0:at * P, (at + 1) * P:n]
+    b.k64[0], b.v64[0], b.lens = k[seen], v[seen], [len(seen)]
+    b.check(got)
+    b.k64[0], b.v64[0], b.lens, b.table = k, v, [n], keep
+    kk, vv = torch.randn(1, heads, D, device=DEV), torch.randn(1, heads, D, device=DEV)
+    kk[0, 0, 3], vv[0, heads - 1, 40] = float("inf"), float("nan")
+    ops.kv_q4_store(b.cache, kk, vv, dev(b.slots(0, np.array([n - 1]))))
+    got = b.run()
+    b.check(got, but=[(new - 1, slice(None))])
+    R = Hq // heads
+    assert torch.isnan(got[new - 1, :R]).all()
+    if heads > 1:
+        last = got[new - 1, -R:]
+        assert torch.isnan(last[:, 32:64]).all() and torch.isfinite(last[:, :32]).all() and torch.isfinite(last[:, 64:]).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_many_rows_whatever_the_workspace_holds(typ):
+    b = Batch(62, 1, 128, 64, [2600, 300, 40], [140, 1, 2], typ, 8)
+    try:
+        for size in (40 << 10, 3 << 20, 9 << 20):
+            torch.cuda.synchronize()
+            ops.shutdown()
+            ops.init(0, size)
+            b.check(b.run())
+    finally:
+        torch.cuda.synchronize()
+        ops.shutdown()
+        ops.init(0, 512 << 20)
+
+
+@pytest.mark.parametrize("Hq,heads", [(1, 1), (64, 1), (96, 1), (200, 1), (24, 8)])
+@pytest.mark.parametrize("typ", ["f32", "f16"])
+@pytest.mark.parametrize("lens,new", [([200], [1]), ([200, 90], [1, 2]), ([300], [9])])
+def test_groups_of_every_size(Hq, heads, typ, lens, new):
+    """One query head per kv head, groups that fill several tiles, and ones past a small request's most rows."""
+    b = Batch(Hq, heads, 64, 64, lens, new, typ, Hq)
+    b.check(b.run())
+    assert status() == 0
+
+
+@pytest.mark.parametrize("typ", list(TYPES))
+@pytest.mark.parametrize("new", [[1, 2], [140, 1]])
+@pytest.mark.parametrize("qmul,kmul,scale", [(1e-4, 1e-3, 2.0**20), (1e-3, 1e3, 1.0), (1e3, 1e-3, 1.0), (1e3, 1e3, 2.0**-20)])
+def test_scales_and_magnitudes(typ, new, qmul, kmul, scale):
+    """kq_scale at both ends of its range, small and large rows, keys behind a row masked all the same."""
+    lens = [200, 40]
+    b = Batch(63, 1, 128, 64, lens, new, typ, 8, qstd=2.0 * qmul, kmul=lambda i, n: np.full(n, kmul))
+    b.check(b.run(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_zero_and_tiny_rows_average_what_they_see(new):
+    b = Batch(64, 1, 64, 32, [170], [new], "f32", 8)
+    for x in (0.0, 1e-38, 1e-30, -1e-25):
+        b.q.fill_(x)
+        b.q64 = np.full(b.q64.shape, np.float64(np.float32(x)))
+        b.check(b.run(scale=2.0**-20), scale=2.0**-20)
+    assert status() == 0
+
+
+def test_many_requests():
+    """The most requests a call takes, some empty, some of many rows."""
+    rng = np.random.default_rng(65)
+    S = 4096
+    lens, new = rng.integers(0, 3, S), np.ones(S, np.int64)
+    new[rng.random(S) < 0.3] = 0
+    lens = np.maximum(lens, new)
+    lens[[5, 2048, 4095]], new[[5, 2048, 4095]] = [90, 150, 40], [80, 70, 33]
+    b = Batch(66, 1, 64, 32, [int(x) for x in lens], [int(x) for x in new], "f16", 4)
+    b.check(b.run(), requests=[0, 1, 2, 3, 5, 63, 64, 65, 2047, 2048, 2049, 4000, 4093, 4094, 4095])
+    assert status() == 0
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_replayed_prefill_beside_other_calls(typ):
+    """A captured call of many rows, replayed after the cache and the lengths it reads have changed and between eager
+    calls that use the same workspace."""
+    b = Batch(67, 1, 128, 64, [1500], [150], typ, 8)
+    other = Batch(68, 1, 128, 64, [4000, 2000], [1, 2], typ, 8)
+    want_other = other.run()
+    out = torch.zeros_like(b.q)
+    table, start, lens = dev(b.table), i32(b.start), i32(b.lens)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.attn_kv_q4(b.cache, b.q, table, start, lens, 150, 1500, out=out)
+    for n in (1500, 700, 1499, 150):
+        lens.copy_(i32([n]))
+        out.zero_()
+        g.replay()
+        assert torch.equal(other.run(), want_other)
+        k, v = b.k64[0], b.v64[0]
+        b.k64[0], b.v64[0], b.lens = k[:n], v[:n], [n]
+        torch.cuda.synchronize()
+        b.check(out)
+        b.k64[0], b.v64[0], b.lens = k, v, [1500]
+    assert status() == 0

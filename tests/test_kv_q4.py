@@ -172,3 +172,25 @@ def test_wrapper_refusals():
         ops.attn_kv_q4(c, torch.zeros(4, 6, 32), i32(2, 3), i32(3), i32(2), 1, 64)
     with pytest.raises(ValueError):
         ops.kv_plan(i32(2), i32(2), i32(3), 32, i32(2, 3), i32(9), torch.zeros(2, dtype=torch.int64), 4)
+
+
+def test_scale_range():
+    for scale in (2.0**-20, 2.0**20, 0.0, 0.125):
+        assert attn(scale=scale) == NOT_READY
+    for scale in (2.0**-21, 2.0**21, 1e-40, 1e30):
+        assert attn(scale=scale) == UNSUPPORTED
+
+
+def test_wrappers_refuse_other_devices(monkeypatch):
+    """Tensors that are not the current device's never reach a kernel (here: host tensors)."""
+    torch = pytest.importorskip("torch")
+    from questwend_amd import ops
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    c = ops.make_kv_q4(torch.zeros(3 * ops.kv_q4_page_bytes(2, 64, 32), dtype=torch.uint8), 2, 64, 32)
+    k, slot = torch.zeros(4, 2, 64), torch.zeros(4, dtype=torch.int64)
+    i32 = lambda *n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    for call in (lambda: ops.kv_q4_store(c, k, k, slot), lambda: ops.kv_q4_load(c, slot),
+                 lambda: ops.attn_kv_q4(c, torch.zeros(4, 6, 64), i32(2, 3), i32(3), i32(2), 1, 64),
+                 lambda: ops.kv_plan(i32(2), i32(2), i32(2), 32, i32(2, 3), i32(9), torch.zeros(2, dtype=torch.int64), 4)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
