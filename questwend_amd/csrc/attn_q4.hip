@@ -315,31 +315,45 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     // rings' last slots, still unused, are)
     _Float16* s_q = (_Float16*) (s_ring + (N - 1) * W * SLOT);
     static_assert(NS * RC * Q4_TILES * LQ * 2 <= W * SLOT, "q fits the last slots");
-    for (int i = w; i < (RC << tshift); i += W) {
-        const bool there = i < rows;
-        const int t = there ? by_R(i) : 0, h = there ? hd * R + i - t * R : 0;
-        constexpr int E = D / 64;                               // values of a lane
-        float x[E], big = 0.0f;
-        const char* src = (const char*) a.q + (int64_t) (s.row0 + t) * a.q_nb1 + (h * D + E * l) * (2 * NS);
+    constexpr int E4 = 4, EV = D / 64;                          // rows of a wave at a time, their values of a lane
+    for (int i0 = w; i0 < (RC << tshift); i0 += E4 * W) {
+        uint8_t raw[E4][EV * 2 * NS];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if constexpr (NS == 2) x[e] = ((const float*) src)[e];
-            else x[e] = a.type == KV_F16 ? (float) ((const _Float16*) src)[e] : bitsf((uint32_t) ((const uint16_t*) src)[e] << 16);
-            big = fmaxf(big, __builtin_fabsf(x[e]));
+        for (int j = 0; j < E4; ++j) {                          // (rows behind the last one: the last one's)
+            const int i = min(i0 + j * W, rows - 1), t = by_R(i), h = hd * R + i - t * R;
+            __builtin_memcpy(raw[j], __builtin_assume_aligned((const char*) a.q + (int64_t) (s.row0 + t) * a.q_nb1 + (h * D + EV * l) * (2 * NS),
+                                                              EV * 2 * NS), EV * 2 * NS);
         }
-        big = max_over_groups(max_over_16(big));
-        // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
-        const int ex = min(max((int) (fbits(big) >> 23) - 127, -60), 127);
-        const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
-        _Float16* dst = s_q + i * LQ + E * l;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float y = there ? x[e] * up : 0.0f;
-            const _Float16 hi = (_Float16) y;
-            dst[e] = hi;
-            if (NS == 2) dst[8 * Q4_TILES * LQ + e] = (_Float16) (y - (float) hi);
+        for (int j = 0; j < E4; ++j) {
+            const int i = i0 + j * W;
+            if (i >= (RC << tshift)) break;
+            float x[EV], big = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EV; ++e) {
+                if constexpr (NS == 2) __builtin_memcpy(&x[e], raw[j] + 4 * e, 4);
+                else {
+                    uint16_t v;
+                    __builtin_memcpy(&v, raw[j] + 2 * e, 2);
+                    x[e] = a.type == KV_F16 ? (float) __builtin_bit_cast(_Float16, v) : bitsf((uint32_t) v << 16);
+                }
+                x[e] = i < rows ? x[e] : 0.0f;
+                big = fmaxf(big, __builtin_fabsf(x[e]));
+            }
+            big = max_over_groups(max_over_16(big));
+            // 2^ex <= big < 2^(ex + 1): q 2^(14 - ex)
+            const int ex = min(max((int) (fbits(big) >> 23) - 127, -60), 127);
+            const float up = bitsf((uint32_t) (127 + 14 - ex) << 23);
+            _Float16* dst = s_q + i * LQ + EV * l;
+#pragma unroll
+            for (int e = 0; e < EV; ++e) {
+                const float y = x[e] * up;
+                const _Float16 hi = (_Float16) y;
+                dst[e] = hi;
+                if (NS == 2) dst[8 * Q4_TILES * LQ + e] = (_Float16) (y - (float) hi);
+            }
+            if (l == 0) s_qs[i] = 512.0f * a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
         }
-        if (l == 0) s_qs[i] = 512.0f * a.scale * bitsf((uint32_t) (127 - 14 + ex) << 23);
     }
     lds_barrier();   // (the cells' copies stay in flight)
     h8 q[NB];

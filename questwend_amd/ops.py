@@ -486,11 +486,14 @@ def _kv_type(dtype) -> int:
     raise TypeError(f"rows of {dtype}: the cache takes float32, float16 and bfloat16")
 
 
-def _kv_here(*tensors) -> None:
-    dev = _torch().cuda.current_device()
+def _kv_stream(*tensors) -> int:
+    """The current stream; the tensors have to be the current device's."""
+    c = _torch()._C
+    dev = tensors[0].get_device()
     for x in tensors:
-        if x.get_device() != dev:   # (-1: host memory)
-            raise ValueError(f"tensors of the current device (cuda:{dev}) are wanted, got one of {x.device}")
+        if dev < 0 or x.get_device() != dev or dev != c._cuda_getDevice():   # (-1: host memory)
+            raise ValueError(f"tensors of the current device are wanted, got one of {x.device}")
+    return c._cuda_getCurrentRawStream(dev)
 
 
 def _kv_rows(x, name: str, T: int, heads: int, D: int) -> int:
@@ -539,14 +542,14 @@ def kv_plan(held, past, new, page_tokens: int, page_table, ring, counters, n_tok
     _kv_index(page_table, "page_table", i32, S, W)
     _kv_index(ring, "ring", i32, n_pages)
     _kv_index(counters, "counters", i64, 2)
-    _kv_here(held, past, new, page_table, ring, counters)
+    st = _kv_stream(held, past, new, page_table, ring, counters)
     dev = held.device
     wide = torch.empty(2 + n_tokens, dtype=i64, device=dev)     # one allocation per type
     narrow = torch.empty(2 * S + 1 + n_tokens, dtype=i32, device=dev)
     out, slot = torch.unsafe_split_with_sizes(wide, (2, n_tokens))   # (half of split()'s time)
     start, length, pos = torch.unsafe_split_with_sizes(narrow, (S + 1, S, n_tokens))
     p8, p4 = wide.data_ptr(), narrow.data_ptr()
-    check(lib().qwmoe_kv_plan(stream(), held.data_ptr(), past.data_ptr(), new.data_ptr(), S, page_tokens, n_pages,
+    check(lib().qwmoe_kv_plan(st, held.data_ptr(), past.data_ptr(), new.data_ptr(), S, page_tokens, n_pages,
                               page_table.data_ptr(), W, ring.data_ptr(), counters.data_ptr(), p8, n_tokens, p4, p4 + 4 * (S + 1),
                               p8 + 16, p4 + 4 * (2 * S + 1)), "kv_plan")
     return out, start, length, slot, pos
@@ -563,8 +566,8 @@ def kv_q4_store(cache: KvQ4, k, v, slot) -> None:
     _kv_index(slot, "slot", _torch().int64, T)
     typ = _kv_type(k.dtype)
     if T:
-        _kv_here(k, v, slot)
-        check(lib().qwmoe_kv_q4_store(stream(), C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
+        st = _kv_stream(k, v, slot)
+        check(lib().qwmoe_kv_q4_store(st, C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
               "kv_q4_store")
 
 
@@ -584,8 +587,8 @@ def kv_q4_load(cache: KvQ4, slot, dtype=None, out=None):
     _kv_index(slot, "slot", torch.int64, T)
     typ = _kv_type(k.dtype)
     if T:
-        _kv_here(k, v, slot)
-        check(lib().qwmoe_kv_q4_load(stream(), C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
+        st = _kv_stream(k, v, slot)
+        check(lib().qwmoe_kv_q4_load(st, C.byref(cache), typ, k.data_ptr(), nbk, v.data_ptr(), nbv, slot.data_ptr(), T),
               "kv_q4_load")
     return k, v
 
@@ -609,8 +612,8 @@ def attn_kv_q4(cache: KvQ4, q, page_table, seq_start, seq_len, max_new: int, max
     _kv_index(seq_len, "seq_len", torch.int32, S)
     typ = _kv_type(q.dtype)
     if T:
-        _kv_here(q, out, page_table, seq_start, seq_len)
-        check(lib().qwmoe_attn_kv_q4(stream(), C.byref(cache), typ, q.data_ptr(), nbq, nq, page_table.data_ptr(), W,
+        st = _kv_stream(q, out, page_table, seq_start, seq_len)
+        check(lib().qwmoe_attn_kv_q4(st, C.byref(cache), typ, q.data_ptr(), nbq, nq, page_table.data_ptr(), W,
                                      seq_start.data_ptr(), seq_len.data_ptr(), S, T, max_new, max_len, scale, out.data_ptr(), nbo),
               "attn_kv_q4")
     return out
