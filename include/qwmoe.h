@@ -599,12 +599,12 @@ int qwmoe_kv_q4_load(void * stream, const qwmoe_kv_q4 * cache, int type, void * 
  * rows the unnormalized weights are rounded to f16 before the sum over the values, and BF16
  * requests of more than 128 rows (n * n_head / n_head_kv) have their keys and values rounded to
  * f16 first.  A NaN or an infinity that was stored shows in the rows that see its
- * block, in no other.  The order of the sums follows max_new, max_len, n_seq, n_tokens and
- * the workspace's size, never the run.
- * Workspace where the keys are split over workgroups, as many splits as fit: per split n_seq *
- * min(max_new, n_tokens, f / (n_head / n_head_kv)) * n_head * (D + 2) floats for requests of up to
- * f rows (64 for F32, else 128), n_tokens * n_head * (D + 2) where there may be longer ones.  A
- * captured call keeps its place in the workspace: no two such calls run at once, and none
+ * block, in no other.  The order of the sums follows the call's sizes and bounds, the
+ * batch's lengths and the workspace's size, never the run.
+ * Workspace where the keys are split over workgroups, as many splits as fit: of n_tokens *
+ * n_head * (D + 2) floats for requests of more than f rows (64 for F32, else 128); for the others
+ * t * n_head * (D + 2) each, t = min(max_new, n_tokens, f / (n_head / n_head_kv)), up to 256 / n_head_kv or
+ * 1.5 n_seq of them and 8 n_seq bytes.  A captured call keeps its place in the workspace: no two such calls run at once, and none
  * after a qwmoe_shutdown or a qwmoe_init that enlarges it. */
 int qwmoe_attn_kv_q4(void * stream, const qwmoe_kv_q4 * cache, int type, const void * q, size_t q_nb1,
                      int64_t n_head, const int32_t * page_table, int64_t table_width, const int32_t * seq_start,

@@ -1147,7 +1147,17 @@ int qwmoe_attn_kv_q4(void* stream, const qwmoe_kv_q4* cache, int type, const voi
         stat = ar.take<float>((size_t) (n * rows * 2));
         return part && stat;
     };
-    if (!split(qw::q4_splits(a), a.S * a.tcap * n_head, a.cells, a.splits, a.part, a.stat) ||
+    a.units = qw::q4_units(a, a.least);
+    if (a.units) {
+        const int64_t rows = a.units * a.tcap * n_head;
+        if ((size_t) (rows * (D + 2)) * 4 + (size_t) a.S * 8 + 2048 <= ar.left()) {
+            a.part = ar.take<float>((size_t) (rows * D));
+            a.stat = ar.take<float>((size_t) (rows * 2));
+            a.first = ar.take<int2>((size_t) a.S);
+            if (!a.part || !a.stat || !a.first) return QWMOE_ERR_WORKSPACE;
+        } else a.units = 0;
+    }
+    if ((!a.units && !split(qw::q4_splits(a), a.S * a.tcap * n_head, a.cells, a.splits, a.part, a.stat)) ||
         !split(qw::q4_row_splits(a), n_tokens * n_head, a.row_cells, a.row_splits, a.row_part, a.row_stat))
         return QWMOE_ERR_WORKSPACE;
     return qw::launch_attn_q4(a, S(stream));

@@ -258,16 +258,50 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     __shared__ float s_qs[RC * Q4_TILES];
     const int tid = threadIdx.x, l = tid & 63, m = l & 15, g = l >> 4;
     const int w = uni(tid >> 6);
-    const int R = a.group, hd = blockIdx.y, z = blockIdx.z;
+    const int R = a.group, hd = blockIdx.y;
     auto by_R = [&](int r) { return R == 1 ? r : (int) __umulhi((unsigned) r, a.group_inv); };   // r / R for 0 <= r < 2^16
+    const int cpp = a.c.page_shift - 5;                         // log2 of a page's cells
+    Q4Seq s;
+    int z, unit;                                                // the split: of the request, and where its sums go
+    int64_t per = a.cells;
+    if (a.units) {
+        // As many cells to a split that the requests' splits are `units` or fewer: a lane has a request.
+        const int i = min(l, a.S - 1), t0 = a.seq_start[i], t1 = a.seq_start[i + 1], n = t1 - t0;
+        s.len = a.seq_len[i];
+        s.n = n;
+        const bool mine = l < a.S && t0 >= 0 && t1 > t0 && t1 <= a.T && (int64_t) n * R <= Q4_TILES * RC;
+        const unsigned c = !mine ? 0 : q4_fits(a, s) ? (unsigned) max((s.len + 31) >> 5, 1) : 1;
+        auto splits = [&](unsigned p) { return (c + p - 1) / p; };
+        auto sum = [&](unsigned v) { return (unsigned) __builtin_amdgcn_readlane((int) kv_wave_incl(v), 63); };
+        const unsigned all = sum(c), units = (unsigned) a.units, spare = units - (unsigned) a.S;
+        // (splits of p cells are at most all / p + S)
+        unsigned lo = max((all - 1) / units + 1, (unsigned) a.least), hi = max((all - 1) / spare + 1, lo);
+        while (lo < hi) {
+            const unsigned p = (lo + hi) / 2;
+            if (sum(splits(p)) <= units) hi = p;
+            else lo = p + 1;
+        }
+        const unsigned mine_n = splits(lo), end = kv_wave_incl(mine_n);
+        const uint64_t has = __ballot(blockIdx.x >= end - mine_n && blockIdx.x < end);
+        if (has == 0) return;
+        const int at = __builtin_ctzll(has);
+        s = Q4Seq{at, __builtin_amdgcn_readlane(n, at), __builtin_amdgcn_readlane(s.len, at), __builtin_amdgcn_readlane(t0, at)};
+        const int before = __builtin_amdgcn_readlane((int) (end - mine_n), at);
+        per = lo;
+        unit = blockIdx.x;
+        z = unit - before;
+        if (z == 0 && hd == 0 && tid == 0) a.first[at] = int2{before, (int) lo};
+    } else {
+        s.i = blockIdx.x;
+        z = blockIdx.z;
+        unit = z * a.S + s.i;
+    }
     // pages of the split's cells, 64 at a time, one per lane (entries behind the request's are read, not used: they
     // come in with its lengths)
-    const int32_t* pages = a.table + (int64_t) blockIdx.x * a.W;
-    const int cpp = a.c.page_shift - 5;                         // log2 of a page's cells
-    const int zc = (int) min((int64_t) z * a.cells, (int64_t) 1 << 30);
+    const int32_t* pages = a.table + (int64_t) s.i * a.W;
+    const int zc = (int) min(z * per, (int64_t) 1 << 30);
     int pg_at = zc >> cpp, pg = pages[min((int64_t) pg_at + l, a.W - 1)];
-    Q4Seq s;
-    if (!q4_request(a, blockIdx.x, s)) return;
+    if (!a.units && !q4_request(a, s.i, s)) return;
     const int rows = (int) min((int64_t) s.n * R, (int64_t) 1 << 30);
     if (rows > Q4_TILES * RC) return;                           // (k_attn_q4_rows')
     int len = s.len;
@@ -286,7 +320,7 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     const int cells = last < 0 ? 0 : (last >> 5) + 1;
     if (z > 0 && zc > (len - 1) >> 5) return;                   // (z = 0 writes the rows without keys)
     const int c0 = min(zc + (w >> tshift), cells);              // its cells: c0, c0 + 2^cshift ..
-    const int c1 = (int) min(zc + a.cells, (int64_t) cells);
+    const int c1 = (int) min(zc + per, (int64_t) cells);
 
     // this lane's row
     const int r = r0 + (m & (RC - 1));
@@ -521,12 +555,12 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
             sum += k < ways ? ol[k].y * f : 0.0f;
         }
         const int tok = by_R(row), hh = hd * R + row - tok * R, lastc = (back + tok) >> 5;
-        if (lastc < a.cells) {          // the row's keys are all in the first split
+        if (lastc < per) {              // the row's keys are all in the first split
             if (z > 0) continue;
             const float inv = sum == 0.0f ? 0.0f : 512.0f / sum;
             q4_put2((char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1, a.type, hh * D + dim, v.x * inv, v.y * inv);
         } else if (zc <= lastc) {
-            const int64_t p = (((int64_t) z * a.S + s.i) * a.tcap + tok) * a.n_head + hh;
+            const int64_t p = ((int64_t) unit * a.tcap + tok) * a.n_head + hh;
             *(float2*) (a.part + p * D + dim) = float2{v.x * 512.0f, v.y * 512.0f};
             if (dim == 0) *(float2*) (a.stat + 2 * p) = float2{at, sum};
         }
@@ -1009,10 +1043,11 @@ template <int D>
 __global__ void __launch_bounds__(256) k_attn_q4_join(AttnQ4Args a, int most) {
     Q4Seq s;
     const int h = blockIdx.y, t = blockIdx.z;
+    const int2 first = a.units ? a.first[blockIdx.x] : int2{(int) blockIdx.x, (int) a.cells};   // (not set: not used)
     if (!q4_request(a, blockIdx.x, s) || t >= s.n || !q4_fits(a, s) || (int64_t) s.n * (a.n_head / a.c.n_head_kv) > most) return;
-    const int parts = q4_parts(s.len - s.n + t, a.cells);
+    const int parts = q4_parts(s.len - s.n + t, first.y);
     if (parts > 1)
-        q4_join<D>(a, s.row0 + t, h, parts, a.part, a.stat, ((int64_t) s.i * a.tcap + t) * a.n_head + h, (int64_t) a.S * a.tcap * a.n_head);
+        q4_join<D>(a, s.row0 + t, h, parts, a.part, a.stat, ((int64_t) first.x * a.tcap + t) * a.n_head + h, (a.units ? 1 : a.S) * a.tcap * a.n_head);
 }
 // of k_attn_q4_rows: workgroups (token row, 1024 / D heads), D / 4 lanes a row: there are rows
 // enough, so each lane adds its splits in order (two splits of 16384 rows of 128: 5.8 us; a
@@ -1040,8 +1075,8 @@ int launch(const AttnQ4Args& a, hipStream_t st) {
     const int few = a.tcap > 0 ? Q4_TILES * (16 / NS) : 0;
     const unsigned nk = (unsigned) a.c.n_head_kv;
     if (few) {
-        hipLaunchKernelGGL((k_attn_q4<D, NS>), dim3((unsigned) a.S, nk, (unsigned) a.splits), dim3(64 * W), 0, st, a);
-        if (a.splits > 1)
+        hipLaunchKernelGGL((k_attn_q4<D, NS>), a.units ? dim3((unsigned) a.units, nk) : dim3((unsigned) a.S, nk, (unsigned) a.splits), dim3(64 * W), 0, st, a);
+        if (a.splits > 1 || a.units)
             hipLaunchKernelGGL(k_attn_q4_join<D>, dim3((unsigned) a.S, (unsigned) a.n_head, (unsigned) a.tcap), dim3(256), 0, st, a, few);
     }
     if (std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) > few) {
@@ -1074,6 +1109,21 @@ int64_t q4_splits(const AttnQ4Args& a) {
     // A workgroup to a CU; twice as many for requests of one tile, which are seldom all as long as the longest
     const int64_t want = a.S > 1 && tiles == 1 ? 512 : 256;
     return std::max<int64_t>(1, std::min<int64_t>({want / groups, cells / (2 * (W / tiles)), 4096}));
+}
+// Requests of several lengths: their cells shared out on the device, to as many workgroups as fit the card once, or in
+// whole rounds of it from half as many again as there are requests on (every request needs one).  us against
+// uniform splits up to max_len: 24 requests of dozens to 8000 keys 11.5 and 17.9, 64 of them 26.6 and 46, 24 of 4000 all 21.0
+// and 24.0, 60 of 2000 all 29 and 25.8.  Up to 64 requests, one to a lane: with four to a lane 200 ragged
+// requests took 48 us, without splits 34, and 24 lost 0.5.
+int q4_units(const AttnQ4Args& a, int& least) {
+    if (q4_few_tokens(a) == 0 || a.S == 1 || a.S > 64) return 0;
+    const int64_t cells = (a.max_len + KV_CELL - 1) / KV_CELL, rows = q4_few_tokens(a) * (a.n_head / a.c.n_head_kv);
+    int tiles = 1;
+    while (tiles < Q4_TILES && (int64_t) tiles * parts_of(a) < rows) tiles *= 2;
+    least = q4_waves(a.c.D) / tiles;
+    if (cells <= 2 * least || a.c.n_head_kv > 256) return 0;
+    const int64_t round = 256 / a.c.n_head_kv;
+    return (int) (round * ((3 * a.S + 2 * round - 1) / (2 * round)));
 }
 int64_t q4_row_blocks(const AttnQ4Args& a) {
     const int per = 8 / qr_halves(a.c.D) * qr_tiles(a.c.D) * 16;

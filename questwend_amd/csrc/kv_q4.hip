@@ -24,22 +24,6 @@ namespace {
 // so the scans stay in registers (DPP adds, one LDS exchange each).  One decode step of 24
 // requests 3.9 us, a round of 512 with 3000 tokens' prompts 6.3 (with 64-bit shuffles
 // 5.0 and 8.6); an empty kernel takes 1.4.
-template <int CTRL, int ROWS = 0xF>
-__device__ __forceinline__ uint32_t kv_dpp(uint32_t v) {
-    return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, ROWS, 0xF, true);
-}
-// Sums that stay at 2^32 - 1 once there: above every bound they are compared with (rows, pages
-// and widths are below 2^31, as is each addend, so a sum that matters is not clipped).
-__device__ __forceinline__ uint32_t kv_add(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
-__device__ __forceinline__ uint32_t kv_wave_incl(uint32_t v) {   // sums over the lanes up to this one
-    v = kv_add(v, kv_dpp<0x111>(v));
-    v = kv_add(v, kv_dpp<0x112>(v));
-    v = kv_add(v, kv_dpp<0x114>(v));
-    v = kv_add(v, kv_dpp<0x118>(v));
-    v = kv_add(v, kv_dpp<0x142, 0xA>(v));   // the last of row 0 to row 1, of row 2 to row 3
-    return kv_add(v, kv_dpp<0x143, 0xC>(v));   // the last of row 1 to rows 2 and 3
-}
-
 __global__ void __launch_bounds__(256) k_kv_plan(KvPlanArgs a) {
     extern __shared__ int32_t s_mem[];
     int32_t* s_start = s_mem;                 // [S + 1] token rows before request i, at most T

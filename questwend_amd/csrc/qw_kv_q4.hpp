@@ -40,6 +40,22 @@ struct KvQ4 {
     }
 };
 
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ uint32_t kv_dpp(uint32_t v) {
+    return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, ROWS, 0xF, true);
+}
+// Sums that stay at 2^32 - 1 once there: above every bound they are compared with (rows, pages
+// and widths are below 2^31, as is each addend, so a sum that matters is not clipped).
+__device__ __forceinline__ uint32_t kv_add(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ uint32_t kv_wave_incl(uint32_t v) {   // sums over the lanes up to this one
+    v = kv_add(v, kv_dpp<0x111>(v));
+    v = kv_add(v, kv_dpp<0x112>(v));
+    v = kv_add(v, kv_dpp<0x114>(v));
+    v = kv_add(v, kv_dpp<0x118>(v));
+    v = kv_add(v, kv_dpp<0x142, 0xA>(v));   // the last of row 0 to row 1, of row 2 to row 3
+    return kv_add(v, kv_dpp<0x143, 0xC>(v));   // the last of row 1 to rows 2 and 3
+}
+
 struct KvPlanArgs {
     const int32_t *held, *past, *n_new;   // [S]
     int S, page_shift;
@@ -87,6 +103,11 @@ struct AttnQ4Args {
     // sums [splits][S][tcap][n_head][D] and [..][2] offset and sum of weights
     int64_t cells, tcap;
     int splits;
+    // or, units > 0: splits by the lengths at hand, `least` cells or more each, `units` of them or fewer for
+    // all requests together; their sums are [units][tcap][n_head][..], a request's first one and cells per split
+    // first[i]
+    int units, least;
+    int2* first;
     float *part, *stat;
     // the others: likewise, [row_splits][T][n_head][..]
     int64_t row_cells;
@@ -96,6 +117,7 @@ struct AttnQ4Args {
 };
 int64_t q4_few_tokens(const AttnQ4Args& a);   // new tokens, at most, of a request of few rows
 int64_t q4_splits(const AttnQ4Args& a);       // splits of the keys that fill the card
+int q4_units(const AttnQ4Args& a, int& least);   // (as in AttnQ4Args)
 int64_t q4_row_splits(const AttnQ4Args& a);
 int64_t q4_row_blocks(const AttnQ4Args& a);
 int launch_attn_q4(const AttnQ4Args& a, hipStream_t stream);

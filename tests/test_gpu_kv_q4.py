@@ -736,3 +736,69 @@ def test_replayed_prefill_beside_other_calls(typ):
         b.check(out)
         b.k64[0], b.v64[0], b.lens = k, v, [1500]
     assert status() == 0
+
+
+# ---- requests whose cells are shared out by the lengths at hand --------------------------
+
+
+@pytest.mark.parametrize("typ,D,heads,Hq", [("f32", 128, 1, 8), ("bf16", 128, 4, 32), ("f16", 64, 2, 14), ("f32", 256, 2, 16)])
+@pytest.mark.parametrize("S", [2, 3, 30, 63, 64, 65])
+def test_ragged_decode(typ, D, heads, Hq, S):
+    """One long request among short ones, idle ones, one of many rows, one without keys, one beyond the bound."""
+    rng = np.random.default_rng(S + D)
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(900), S)).astype(int)]
+    new = [1] * S
+    lens[S // 2] = 2777
+    if S > 3:
+        lens[1], new[2], lens[3], new[4], lens[4] = 0, 0, 3, 5, 700
+    if S == 30:
+        lens[7], new[7] = 300, 260                      # (many rows)
+    b = Batch(70 + S, heads, D, 64, lens, new, typ, Hq, pad=2)
+    out = torch.full_like(b.q, 5.0)
+    b.run(out=out)
+    b.check(out)
+    assert status() == 0
+    assert torch.equal(out[b.start[-1]:], torch.full_like(out[b.start[-1]:], 5.0))
+    first = out.clone()
+    b.run(out=out)
+    assert torch.equal(out, first)
+    got = b.run(max_len=2776, max_new=max(new))         # the long one is beyond the bound
+    assert status() == qa.STATUS_BAD_SEQ
+    i = int(b.start[S // 2])
+    assert torch.count_nonzero(got[i:i + 1]) == 0
+    b.check(got, requests=[x for x in range(S) if x != S // 2])
+
+
+def test_ragged_lengths_change_between_replays():
+    """The shares follow the lengths on the device: one captured call over several sets of them."""
+    lens, new = [3000, 40, 700, 1, 90, 2000], [1, 2, 1, 1, 3, 1]
+    b = Batch(71, 2, 128, 64, lens, new, "f32", 16)
+    out = torch.zeros_like(b.q)
+    table, start, there = dev(b.table), i32(b.start), i32(lens)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.attn_kv_q4(b.cache, b.q, table, start, there, 3, 3000, out=out)
+    k, v = b.k64, b.v64
+    for now in (lens, [1, 1, 1, 1, 3, 1], [10, 33, 700, 0, 64, 1999], [3000, 40, 1, 1, 5, 2], [0] * 6, lens):
+        there.copy_(i32(now))
+        out.fill_(9.0)
+        g.replay()
+        (torch.randn(1000, device=DEV) ** 2).sum().item()
+        torch.cuda.synchronize()
+        b.k64, b.v64, b.lens = [x[:n] for x, n in zip(k, now)], [x[:n] for x, n in zip(v, now)], now
+        b.check(out)
+    assert status() == 0
+
+
+def test_ragged_lengths_in_odd_orders():
+    """Rows of seq_start that lie outside the call or fall back leave the other requests as they are."""
+    b = Batch(72, 1, 64, 64, [900, 500, 40], [1, 1, 1], "f16", 8)
+    want = b.run()
+    for start in ([0, 1, 2, 2], [0, 1, 2, 9], [0, 1, 2, 0]):
+        out = torch.full_like(b.q, 5.0)
+        b.start = np.array(start)
+        b.run(out=out)
+        assert torch.equal(out[2], torch.full_like(out[2], 5.0))
+        for i in (0, 1):
+            w, o = want[i].double(), out[i].double()
+            assert float((w - o).abs().max()) <= 2.0**-8 * float(w.abs().max())   # (shares, so sums' orders, differ)
