@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     }
     // the waves of the workgroup: 2^tshift tiles of rows, 2^cshift waves each
     const int tshift = rows <= RC ? 0 : rows <= 2 * RC ? 1 : rows <= 4 * RC ? 2 : 3;
-    const int cshift = (W == 16 ? 4 : 3) - tshift;
+    const int cshift = 3 - tshift;
     const int r0 = (w & ((1 << tshift) - 1)) * RC;              // the wave's first row
     const int wrows = max(min(rows - r0, RC), 0);
     const int back = len - s.n;                                 // a row of token t sees keys .. back + t
@@ -532,38 +532,47 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     if (m < RC)
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) *(f4*) (s_o + (w * RC + m) * LD + 16 * i + 4 * g) = o[i];
-    const int ways = 1 << cshift, tiles = 1 << tshift;
+    const int tiles = 1 << tshift;
     __syncthreads();
-    for (int e = tid; e < rows * (D / 2); e += 64 * W) {
-        const int row = e / (D / 2), dim = 2 * (e % (D / 2)), tile = row / RC, rr = row % RC;
-        float2 ol[W], part[W];
+    auto join = [&](auto ways_) __attribute__((always_inline)) {
+        constexpr int ways = decltype(ways_)::value;
+        for (int e = tid; e < rows * (D / 2); e += 64 * W) {
+            const int row = e / (D / 2), dim = 2 * (e % (D / 2)), tile = row / RC, rr = row % RC;
+            float2 ol[ways], part[ways];
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            const int from = tile + tiles * (k & (ways - 1));
-            ol[k] = s_ol[from][rr];
-            part[k] = *(const float2*) (s_o + (from * RC + rr) * LD + dim);
-        }
-        float at = ol[0].x, sum = 0.0f;
+            for (int k = 0; k < ways; ++k) {
+                const int from = tile + tiles * k;
+                ol[k] = s_ol[from][rr];
+                part[k] = *(const float2*) (s_o + (from * RC + rr) * LD + dim);
+            }
+            float at = ol[0].x, sum = 0.0f;
 #pragma unroll
-        for (int k = 1; k < W; ++k) at = fmaxf(at, ol[k].x);
-        float2 v = float2{0.0f, 0.0f};
+            for (int k = 1; k < ways; ++k) at = fmaxf(at, ol[k].x);
+            float2 v = float2{0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            const float f = k < ways ? exp2_hw(ol[k].x - at) : 0.0f;
-            v.x += k < ways ? part[k].x * f : 0.0f;   // (0 times a NaN)
-            v.y += k < ways ? part[k].y * f : 0.0f;
-            sum += k < ways ? ol[k].y * f : 0.0f;
+            for (int k = 0; k < ways; ++k) {
+                const float f = exp2_hw(ol[k].x - at);
+                v.x += part[k].x * f;
+                v.y += part[k].y * f;
+                sum += ol[k].y * f;
+            }
+            const int tok = by_R(row), hh = hd * R + row - tok * R, lastc = (back + tok) >> 5;
+            if (lastc < per) {              // the row's keys are all in the first split
+                if (z > 0) continue;
+                const float inv = sum == 0.0f ? 0.0f : 512.0f / sum;
+                q4_put2((char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1, a.type, hh * D + dim, v.x * inv, v.y * inv);
+            } else if (zc <= lastc) {
+                const int64_t p = ((int64_t) unit * a.tcap + tok) * a.n_head + hh;
+                *(float2*) (a.part + p * D + dim) = float2{v.x * 512.0f, v.y * 512.0f};
+                if (dim == 0) *(float2*) (a.stat + 2 * p) = float2{at, sum};
+            }
         }
-        const int tok = by_R(row), hh = hd * R + row - tok * R, lastc = (back + tok) >> 5;
-        if (lastc < per) {              // the row's keys are all in the first split
-            if (z > 0) continue;
-            const float inv = sum == 0.0f ? 0.0f : 512.0f / sum;
-            q4_put2((char*) a.out + (int64_t) (s.row0 + tok) * a.out_nb1, a.type, hh * D + dim, v.x * inv, v.y * inv);
-        } else if (zc <= lastc) {
-            const int64_t p = ((int64_t) unit * a.tcap + tok) * a.n_head + hh;
-            *(float2*) (a.part + p * D + dim) = float2{v.x * 512.0f, v.y * 512.0f};
-            if (dim == 0) *(float2*) (a.stat + 2 * p) = float2{at, sum};
-        }
+    };
+    switch (cshift) {
+        case 0: join(std::integral_constant<int, 1>()); break;
+        case 1: join(std::integral_constant<int, 2>()); break;
+        case 2: join(std::integral_constant<int, 4>()); break;
+        default: join(std::integral_constant<int, 8>());
     }
 }
 
