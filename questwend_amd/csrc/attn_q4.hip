@@ -130,12 +130,19 @@ __device__ __forceinline__ float half_of(uint32_t w, int hi) {
     __builtin_memcpy(&x, &w, 4);
     return (float) x[hi];
 }
-// v less the low or high half of w, in one instruction
+// v less the low or high half of w, in one instruction; or plus s times it
 template <int HIGH>
 __device__ __forceinline__ float less_half(float v, uint32_t w) {
     float r;
     if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(v));
     else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(v));
+    return r;
+}
+template <int HIGH>
+__device__ __forceinline__ float plus_half(float v, uint32_t w, float s) {
+    float r;
+    if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(s), "v"(v));
+    else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(w), "v"(s), "v"(v));
     return r;
 }
 __device__ __forceinline__ uint32_t word_of(_Float16 lo, _Float16 hi) {
@@ -406,7 +413,7 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     int E = -25;                 // the value scales so far are at most 2^E
     int Ebits = 0;               // 2^E as f16 bits
 
-    const uint32_t high = m < RC ? 0xffffffffu : 0u;            // lanes with high parts
+    const float less = m < RC ? 0.0f : -1.0f;                   // (lanes with low parts: what the high one leaves)
     int slot = 0;
     for (int c = c0; c < c1; c += 1 << cshift) {
         const int ahead = c + ((N - 1) << cshift);
@@ -498,12 +505,7 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
                     float w0 = __builtin_fmaf(p0, d0, 0.0f), w1 = __builtin_fmaf(p1, d1, 0.0f);
                     asm volatile("" : "+v"(w0), "+v"(w1));
                     uint32_t hi = word_of((_Float16) w0, (_Float16) w1);
-                    if (NS == 2) {
-                        asm volatile("" : "+v"(hi));
-                        float v0 = __builtin_fmaf(p0, d0, -half_of(hi, 0)), v1 = __builtin_fmaf(p1, d1, -half_of(hi, 1));
-                        asm volatile("" : "+v"(v0), "+v"(v1));
-                        hi = (hi & high) | (word_of((_Float16) v0, (_Float16) v1) & ~high);
-                    }
+                    if (NS == 2) hi = word_of((_Float16) plus_half<0>(w0, hi, less), (_Float16) plus_half<1>(w1, hi, less));
                     pw[k] = hi;
                 }
                 if (masked)   // (a masked key's scale may be a NaN)
