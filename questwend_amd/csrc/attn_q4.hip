@@ -3,12 +3,15 @@
 // 0 .. len - n + t,
 //   o = sum_j softmax_j(scale q . k_j) v_j.
 //
-// Codes become f16 operands of v_mfma_f32_16x16x32_f16 in registers, without LDS: a code
-// masked out of its dword is the f16 subnormal c 2^-24 (or, a nibble further on, c 2^-20), for
+// Requests of few rows (decode steps, drafts) are k_attn_q4's, requests of many (chunks of a prompt) are
+// k_attn_q4_rows', which has its own notes.  Both form f16 operands of v_mfma_f32_16x16x32_f16 in
+// registers: a code masked out of its dword is the f16 subnormal c 2^-24 (or, a nibble further on, c 2^-20), for
 // two codes at once, and one packed multiply-add makes that (c - 8) 2^-9, exactly: nine
 // instructions for eight operands.  (The subnormals themselves multiply too, but the
-// products' sum then keeps 16 bits only.)  Block scales are applied in fp32 around
-// the products, so the cache's values enter unrounded:
+// products' sum then keeps 16 bits only.)
+//
+// Few rows: block scales are applied in fp32 around the products, so the cache's values enter
+// unrounded:
 //   scores   S^T = K Q^T, 16 keys x 16 rows, 32 dims (one block) a product; each block's
 //            product is scaled by d_k of (key, block) as it is added;
 //   values   O^T = V^T P^T, 16 dims x 16 rows, 32 keys a product, P's entries times d_v of (key,
@@ -29,9 +32,18 @@
 // or some scale 2^E.  Otherwise a cell costs no exchange between lanes and no rescaling.
 //
 // A workgroup takes a request's rows (R = n_head / n_head_kv per token), one kv head and one
-// split of the keys.  Its waves share out 16-column tiles of the rows, and waves of the
-// same tile share out the cells; their sums meet in LDS, the splits' in a second launch.
-// The next cell's dwords are loaded while this one's are computed on.
+// split of the keys.  Its eight waves share out 16-column tiles of the rows, and waves of the
+// same tile share out the cells; their sums meet in LDS, the splits' in a second launch.  Each
+// wave copies its next cells straight into its own ring in LDS (no registers, no barrier: a wave
+// waits for its own copies only), and the rings take what LDS there is: a workgroup to a CU.
+//
+// What bounds it: a long context reads its cells at the card's rate (one row of 131072 keys, four kv heads of 128,
+// 75 MB: 24.0 us, about 4 of them before the first cell is there, and 4.4 for the join; a large sum reads 3.9 TB/s
+// here); shorter ones wait for a chain of loads, lengths -> pages -> cells, and for each wave's 400 vector instructions
+// a cell: one row of 700 keys 11.3 us, of which an empty kernel is 1.4; 24 requests of dozens to 8000 keys, 16 MB,
+// 11.5 + 4.0; eight requests' five rows of up to 3000 keys at D = 256 16.6 + 6.3.  Against it: cells loaded into
+// registers instead of the rings 35 us for the long context, 14.9 for the 700 keys; sixteen waves a workgroup, with
+// half the registers each, slower.
 #include <algorithm>
 #include <type_traits>
 
@@ -202,7 +214,7 @@ __device__ __forceinline__ int max_of_wave(int v) {
 // (lane l ^ 8 of the same 16)
 __device__ __forceinline__ float other_part(float v) { return dpp_f<0x128>(v); }   // row_ror:8
 
-// Waves of a workgroup: as many as the registers hold, a workgroup to a CU.  Cells of a wave in flight or in
+// Waves of a workgroup: two to a SIMD (more have too few registers, and each brings its own q and sums).  Cells of a wave in flight or in
 // use: as many as LDS holds.
 constexpr int q4_waves(int D) { return 8; }
 constexpr int q4_ring(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
@@ -589,13 +601,26 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
 // that only fall, where some cell's largest scale asks for it (every wave looks at every
 // scale, so all agree without exchange).
 //
+// f32 rows are two f16 parts in separate operands: of the four products of parts, low by low is left out
+// (2^-24 of the whole, a step of fp32).
+//
 // D <= 128: four waves' rows, two tiles each, and two cells at a time, one per half of the waves,
 // whose sums meet in LDS at the end; D = 256: eight waves' rows, a tile each, one cell at a time.
 // Two buffers: the next step's operands are formed, and the one after's dwords loaded, while this
-// one's are used; one barrier a step.
+// one's are used; one barrier a step.  One of a SIMD's two waves forms while the other multiplies.
+//
+// What bounds it: the instructions around the products.  A wave's 64 keys take 96 products (f32 rows, D = 128: 1600
+// clocks alone), about 130 vector instructions to form its share of the operands and 100 for two tiles' softmax, at 4 clocks
+// and more each beside a product; measured 2.9 us a step where the products of both waves need 1.5.  A chunk of
+// 512 tokens behind 1037 (32 heads on 4, D = 128): f32 49.5 us + 5.8 to join two splits, f16 43 + 5.2, bf16 37 + 5.2;
+// one of 1024 bf16 tokens up to 4000 keys 109 us (58.8 Gflop, 540 Tflop/s).  Of a chunk's time about 12 us lie before
+// the first product (lengths, pages, q) and behind the last (sums, output).  Tried and slower: four waves to a SIMD
+// with a tile each (f32 63.8 us: spills), the next operands formed between this step's products in one wave (54.0),
+// one tile a wave (58.8 unsplit).
 //
 // A NaN scale of a value is taken as 0 and its block set to NaN afterwards in the rows that
 // see the key: 0 times NaN would reach those that do not.
+// (16 x 16 tiles of a wave, halves of the workgroup: what 256 registers and 160 KiB of LDS hold)
 constexpr int qr_tiles(int D) { return D == 256 ? 1 : 2; }
 constexpr int qr_halves(int D) { return D == 256 ? 1 : 2; }
 
@@ -1079,7 +1104,8 @@ __global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int mos
     q4_put4((char*) a.out + (int64_t) tok * a.out_nb1, a.type, h * D + dim, v.value());
 }
 
-// Requests of up to `few` rows are k_attn_q4's, the others k_attn_q4_rows' (a lone request that may have more rows: too).
+// Requests of up to `few` rows (eight tiles) are k_attn_q4's, the others k_attn_q4_rows', each kernel passing over the
+// other's.  A lone request that may have more rows is k_attn_q4_rows' whatever it has: one launch, not two.
 template <int D, int NS>
 int launch(const AttnQ4Args& a, hipStream_t st) {
     constexpr int W = q4_waves(D);
@@ -1117,9 +1143,10 @@ int64_t q4_splits(const AttnQ4Args& a) {
     const int64_t rows = q4_few_tokens(a) * (a.n_head / a.c.n_head_kv), W = q4_waves(a.c.D);
     int64_t tiles = 1;
     while (tiles < Q4_TILES && tiles * parts_of(a) < rows) tiles *= 2;
-    // A workgroup to a CU; twice as many for requests of one tile, which are seldom all as long as the longest
+    // A workgroup to a CU (512: 131072 keys 29.2 us instead of 24.0), but twice as many for several requests of one tile, which
+    // are seldom all as long as the longest (256: 24 ragged requests 26 us instead of 17.9); two cells to a wave at least.
     const int64_t want = a.S > 1 && tiles == 1 ? 512 : 256;
-    return std::max<int64_t>(1, std::min<int64_t>({want / groups, cells / (2 * (W / tiles)), 4096}));
+    return std::max<int64_t>(1, std::min<int64_t>(want / groups, cells / (2 * (W / tiles))));
 }
 // Requests of several lengths: their cells shared out on the device, to as many workgroups as fit the card once, or in
 // whole rounds of it from half as many again as there are requests on (every request needs one).  us against
@@ -1142,6 +1169,8 @@ int64_t q4_row_blocks(const AttnQ4Args& a) {
 }
 int64_t q4_row_splits(const AttnQ4Args& a) {
     if (std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) <= few_of(a)) return 1;
+    // As near to a workgroup per CU as whole splits come, of eight cells at least.  A 512-token f32 chunk in 2 splits (264
+    // workgroups): 49.5 + 5.8 us, in 3 68.8 + 6.9, in 1 75; 100 tokens in 6 splits of 8 cells 27.7 + 4.7, in 3 of 16 35.8 + 4.6.
     const int64_t groups = q4_row_blocks(a) * a.c.n_head_kv, cells = (a.max_len + KV_CELL - 1) / KV_CELL;
     return std::max<int64_t>(1, std::min<int64_t>((256 + groups / 2) / groups, cells / 8));
 }
