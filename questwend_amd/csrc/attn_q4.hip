@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
         const int i = min(l, a.S - 1), t0 = a.seq_start[i], t1 = a.seq_start[i + 1], n = t1 - t0;
         s.len = a.seq_len[i];
         s.n = n;
-        const bool mine = l < a.S && t0 >= 0 && t1 > t0 && t1 <= a.T && (int64_t) n * R <= Q4_TILES * RC;
+        const bool mine = l < a.S && t0 >= 0 && t1 > t0 && t1 <= a.T && (n > a.max_new || (int64_t) n * R <= Q4_TILES * RC);
         const unsigned c = !mine ? 0 : q4_fits(a, s) ? (unsigned) max((s.len + 31) >> 5, 1) : 1;
         auto splits = [&](unsigned p) { return (c + p - 1) / p; };
         auto sum = [&](unsigned v) { return (unsigned) __builtin_amdgcn_readlane((int) kv_wave_incl(v), 63); };
@@ -322,6 +322,15 @@ __global__ void __launch_bounds__(64 * q4_waves(D)) __attribute__((amdgpu_waves_
     int pg_at = zc >> cpp, pg = pages[min((int64_t) pg_at + l, a.W - 1)];
     if (!a.units && !q4_request(a, s.i, s)) return;
     const int rows = (int) min((int64_t) s.n * R, (int64_t) 1 << 30);
+    if (s.n > a.max_new) {                                      // however many rows: zeros
+        if (z > 0) return;
+        if (tid == 0) atomicOr(a.status, QWMOE_STATUS_BAD_SEQ);
+        for (int64_t e = tid; e < (int64_t) s.n * R * (D / 4); e += 64 * W) {
+            const int64_t row = e / (D / 4);
+            q4_put4((char*) a.out + (s.row0 + row / R) * a.out_nb1, a.type, (hd * R + row % R) * D + 4 * (e % (D / 4)), f4{0.0f, 0.0f, 0.0f, 0.0f});
+        }
+        return;
+    }
     if (rows > Q4_TILES * RC) return;                           // (k_attn_q4_rows')
     int len = s.len;
     if (!q4_fits(a, s)) {
@@ -661,7 +670,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))
     Q4Seq s;
     if (!q4_find(a, l, blockIdx.x, [&](int t, int i) { return (int64_t) max(t, 0) * R / RB + i; }, s)) return;
     const int rows = (int) min((int64_t) s.n * R, (int64_t) 1 << 30);
-    if (rows <= most) return;                                   // (k_attn_q4's)
+    if (rows <= most || (most && s.n > a.max_new)) return;      // (k_attn_q4's)
     // the request's blocks, the last rows (the most keys) first
     const int blocks = (rows + RB - 1) / RB, at = blockIdx.x - (int) ((int64_t) s.row0 * R / RB + s.i);
     if (at >= blocks) return;
@@ -1105,7 +1114,8 @@ __global__ void __launch_bounds__(256) k_attn_q4_rows_join(AttnQ4Args a, int mos
 }
 
 // Requests of up to `few` rows (eight tiles) are k_attn_q4's, the others k_attn_q4_rows', each kernel passing over the
-// other's.  A lone request that may have more rows is k_attn_q4_rows' whatever it has: one launch, not two.
+// other's; one beyond max_new is k_attn_q4's where that runs.  A lone request that may have more rows is
+// k_attn_q4_rows' whatever it has: one launch, not two.
 template <int D, int NS>
 int launch(const AttnQ4Args& a, hipStream_t st) {
     constexpr int W = q4_waves(D);
@@ -1116,7 +1126,7 @@ int launch(const AttnQ4Args& a, hipStream_t st) {
         if (a.splits > 1 || a.units)
             hipLaunchKernelGGL(k_attn_q4_join<D>, dim3((unsigned) a.S, (unsigned) a.n_head, (unsigned) a.tcap), dim3(256), 0, st, a, few);
     }
-    if (std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) > few) {
+    if (few == 0 || std::min(a.max_new, a.T) * (a.n_head / a.c.n_head_kv) > few) {
         const int64_t blocks = q4_row_blocks(a);
         if (blocks > 0x7fffffff) return -2;
         const dim3 g((unsigned) blocks, nk, (unsigned) a.row_splits);

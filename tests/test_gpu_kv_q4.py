@@ -802,3 +802,40 @@ def test_ragged_lengths_in_odd_orders():
         for i in (0, 1):
             w, o = want[i].double(), out[i].double()
             assert float((w - o).abs().max()) <= 2.0**-8 * float(w.abs().max())   # (shares, so sums' orders, differ)
+
+
+@pytest.mark.parametrize("typ", list(TYPES))
+@pytest.mark.parametrize("D,heads,Hq", [(128, 1, 8), (64, 2, 4), (256, 1, 3)])
+@pytest.mark.parametrize("lens,new,max_new", [([90, 300, 200], [1, 140, 2], 2), ([300, 90], [200, 1], 1), ([300], [260], 1),
+                                              ([400, 300, 90], [300, 150, 1], 150), ([90, 40], [2, 3], 0), ([300], [150], 0)])
+def test_many_rows_beyond_max_new(typ, D, heads, Hq, lens, new, max_new):
+    """A request of more rows than the bound names gets zeros and a status, however many they are; the others their result."""
+    b = Batch(80, heads, D, 64, lens, new, typ, Hq, pad=2)
+    out = torch.full_like(b.q, 5.0)
+    b.run(out=out, max_new=max_new)
+    assert status() == qa.STATUS_BAD_SEQ
+    for i, n in enumerate(new):
+        if n > max_new:
+            assert torch.count_nonzero(out[b.start[i]:b.start[i + 1]]) == 0
+    b.check(out, requests=[i for i, n in enumerate(new) if n <= max_new])
+    assert torch.equal(out[b.start[-1]:], torch.full_like(out[b.start[-1]:], 5.0))
+
+
+@pytest.mark.parametrize("new", [[1], [1, 3], [150, 1]])
+def test_no_keys_at_all(new):
+    b = Batch(81, 1, 128, 32, [0] * len(new), new, "bf16", 8)
+    out = torch.full_like(b.q, 5.0)
+    b.run(out=out, max_len=0)
+    assert torch.count_nonzero(out) == 0 and status() == 0
+
+
+def test_requests_that_share_pages():
+    """Two requests over one prefix's pages, and a page that occurs twice in a request."""
+    b = Batch(82, 2, 128, 64, [192, 200, 192], [1, 4, 130], "f32", 8)
+    b.table[1, :2] = b.table[0, :2]
+    b.table[2, 2] = b.table[2, 0]
+    for x in (b.k64, b.v64):
+        x[1][:128] = x[0][:128]
+        x[2][128:] = x[2][:64]
+    b.check(b.run())
+    assert status() == 0
