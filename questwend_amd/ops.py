@@ -490,10 +490,13 @@ def _kv_stream(*tensors) -> int:
     """The current stream; the tensors have to be the current device's."""
     c = _torch()._C
     dev = tensors[0].get_device()
-    for x in tensors:
-        if dev < 0 or x.get_device() != dev or dev != c._cuda_getDevice():   # (-1: host memory)
-            raise ValueError(f"tensors of the current device are wanted, got one of {x.device}")
-    return c._cuda_getCurrentRawStream(dev)
+    if dev >= 0 and dev == c._cuda_getDevice():   # (-1: host memory)
+        for x in tensors:
+            if x.get_device() != dev:
+                break
+        else:
+            return c._cuda_getCurrentRawStream(dev)
+    raise ValueError(f"tensors of the current device are wanted, got {[str(x.device) for x in tensors]}")
 
 
 def _kv_rows(x, name: str, T: int, heads: int, D: int) -> int:
@@ -577,13 +580,15 @@ def kv_q4_load(cache: KvQ4, slot, dtype=None, out=None):
     torch = _torch()
     T, heads, D = slot.shape[0], cache.n_head_kv, cache.n_embd_head
     if out is None:
-        k, v = torch.empty((2, T, heads, D), dtype=dtype or torch.float32, device=slot.device).unbind(0)
+        both = torch.empty((2 * T, heads, D), dtype=dtype or torch.float32, device=slot.device)   # one allocation
+        k, v = torch.unsafe_split_with_sizes(both, (T, T))
+        nbk = nbv = heads * D * k.element_size()
     else:
         k, v = out
-    nbk = _kv_rows(k, "k", T, heads, D)
-    nbv = _kv_rows(v, "v", T, heads, D)
-    if v.dtype is not k.dtype:
-        raise ValueError("k and v: one type is wanted")
+        nbk = _kv_rows(k, "k", T, heads, D)
+        nbv = _kv_rows(v, "v", T, heads, D)
+        if v.dtype is not k.dtype:
+            raise ValueError("k and v: one type is wanted")
     _kv_index(slot, "slot", torch.int64, T)
     typ = _kv_type(k.dtype)
     if T:
