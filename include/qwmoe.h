@@ -602,10 +602,11 @@ int qwmoe_kv_q4_load(void * stream, const qwmoe_kv_q4 * cache, int type, void * 
  * block, in no other.  The order of the sums follows the call's sizes and bounds, the
  * batch's lengths and the workspace's size, never the run.
  * Workspace where the keys are split over workgroups, as many splits as fit: of n_tokens *
- * n_head * (D + 2) floats for requests of more than f rows (64 for F32, else 128); for the others
- * t * n_head * (D + 2) each, t = min(max_new, n_tokens, f / (n_head / n_head_kv)), up to 256 / n_head_kv or
- * 1.5 n_seq of them and 8 n_seq bytes.  A captured call keeps its place in the workspace: no two such calls run at once, and none
- * after a qwmoe_shutdown or a qwmoe_init that enlarges it. */
+ * n_head * (D + 2) floats for requests of more than f rows (64 for F32, else 128); for the
+ * others t * n_head * (D + 2) each, t = min(max_new, n_tokens, f / (n_head / n_head_kv)), up to
+ * 256 / n_head_kv or 1.5 n_seq of them, and 8 n_seq bytes.  A captured call keeps its place in
+ * the workspace: no two such calls run at once, and none after a qwmoe_shutdown or a
+ * qwmoe_init that enlarges it. */
 int qwmoe_attn_kv_q4(void * stream, const qwmoe_kv_q4 * cache, int type, const void * q, size_t q_nb1,
                      int64_t n_head, const int32_t * page_table, int64_t table_width, const int32_t * seq_start,
                      const int32_t * seq_len, int64_t n_seq, int64_t n_tokens, int64_t max_new, int64_t max_len,
